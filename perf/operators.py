@@ -268,7 +268,7 @@ def _plain_log_probs(s, case):
 
 def _plain_policy_loss(s, case):
     lp, adv, w = s["log_probs"].float(), s["advantage"], s["mask"].float()
-    low, high = 0.2, case["high"] if case["variant"] == "clip" else 0.2
+    low, high = 0.2, case["high"]
     # 64 bits next to a border of the clip and where exp(x) - 1 - x cancels
     log_w = s["log_probs"].double() - s["old"].double()
     above, below = log_w > math.log1p(high), log_w < math.log1p(-low)
@@ -437,7 +437,7 @@ def _exact_policy_loss(s, case):
         if case["variant"] == "clip":
             gain = torch.minimum(log_w.exp() * adv, log_w.exp().clamp(0.8, 1 + case["high"]) * adv)
         else:
-            gain = log_w.exp().detach().clamp(0.8, 1.2) * log_w * adv
+            gain = log_w.exp().detach().clamp(0.8, 1 + case["high"]) * log_w * adv
         objective = -gain[keep].sum() / count
         kl = torch.zeros((), dtype=torch.float64, device=lp.device)
         if s["ref"] is not None:
