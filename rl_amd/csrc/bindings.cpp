@@ -9,6 +9,7 @@
 
 #include <vector>
 
+#include "llm_bindings.h"
 #include "segment_tree_cpu.h"
 
 #ifdef RL_AMD_WITH_HIP
@@ -1350,6 +1351,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 #endif
 
   rl_amd::define_segment_trees(m);
+  rl_amd::define_language_ops(m);
   m.def("safetanh", &safetanh_fwd, "clamped tanh");
   m.def("safeatanh", &safeatanh_fwd, "clamped atanh");
 

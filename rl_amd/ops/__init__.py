@@ -1211,3 +1211,13 @@ def fuse_mlp3(module: torch.nn.Module) -> torch.nn.Module:
     ):
         return FusedMLP3(*linears, eager=module)
     return module
+
+
+from .language import (  # noqa: E402
+    TokenPolicyLoss,
+    paged_attention_decode,
+    paged_kv_append,
+    rotary_table,
+    token_log_probs,
+    token_policy_loss,
+)

@@ -19,7 +19,10 @@ CSRC = os.path.join(ROOT, "rl_amd", "csrc")
 
 with_hip = torch.version.hip is not None
 
-sources = [os.path.join(CSRC, "bindings.cpp")]
+sources = [
+    os.path.join(CSRC, "bindings.cpp"),
+    os.path.join(CSRC, "llm_bindings.cpp"),
+]
 extra_cflags = ["-O3", "-std=c++17"]
 define_macros = []
 
@@ -34,13 +37,20 @@ if with_hip:
         os.path.join(CSRC, "loss_ops.hip"),
         os.path.join(CSRC, "fused_mlp.hip"),
         os.path.join(CSRC, "rollout_fused.hip"),
+        os.path.join(CSRC, "token_loss.hip"),
+        os.path.join(CSRC, "paged_kv.hip"),
     ]
     define_macros.append(("RL_AMD_WITH_HIP", None))
     ext_cls = cpp_extension.CUDAExtension
     extra = {
         "extra_compile_args": {
             "cxx": extra_cflags,
-            "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+            # no packed fp32 instructions: some of their forms have given wrong
+            # results on this hardware now and then
+            "nvcc": [
+                "-O3", "-std=c++17", "--offload-arch=gfx950",
+                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+            ],
         }
     }
 else:

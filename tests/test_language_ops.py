@@ -1,0 +1,703 @@
+"""The language-model operators against plain 64-bit forms.
+
+``u = 2**-24`` is half a step of float32; an output rounded to ``dtype`` is off
+by at most ``finfo(dtype).eps / 2`` of its value (plus half a subnormal step).
+"""
+import math
+
+import pytest
+import torch
+
+from rl_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+U = 2.0 ** -24
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def half_step(ref, dtype):
+    info = torch.finfo(dtype)
+    return ref.abs() * info.eps / 2 + info.tiny * info.eps / 2
+
+
+def close(got, ref, tol):
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape
+    assert torch.equal(got.isnan(), ref.isnan())
+    ok = ref.isnan() | (got == ref) | ((got - ref).abs() <= tol)
+    assert ok.all(), ((got - ref).abs() - tol)[~ok].max()
+
+
+# --------------------------------------------------------------------------- #
+# token_log_probs
+# --------------------------------------------------------------------------- #
+def log_probs_oracle(logits, tokens, temperature, ignore, upstream):
+    z = logits.detach().cpu().double() / temperature
+    tokens = tokens.cpu().long()
+    live = tokens != ignore
+    p = torch.softmax(z, -1)
+    at = torch.where(live, tokens, 0).unsqueeze(-1)
+    lp = torch.where(live, torch.log_softmax(z, -1).gather(-1, at).squeeze(-1), 0.0)
+    g = torch.where(live, upstream.cpu().double() / temperature, 0.0).unsqueeze(-1)
+    grad = torch.where(g == 0, 0.0, -g * p)
+    grad.scatter_add_(-1, at, g)
+    return lp, grad, g, p, z
+
+
+def log_probs_tolerance(z, g, p, grad, vocab, dtype):
+    """Relative error of one exp: its argument (z - m) / T * log2(e) is rounded
+    three times, which the exponential turns into 3 u |z - m| / T, and the
+    instruction adds 2 u.  Terms far below the maximum weigh nothing, so
+    |z - m| / T <= 40 is what counts.  A thread adds at most vocab / 64 terms
+    in a row, each rounded.  log and the last sum round the result itself."""
+    far = (z.amax(-1, keepdim=True) - z).clamp(max=40).amax(-1, keepdim=True)
+    rel = U * (6 * far + vocab / 64 + 32)
+    size = (z.amax(-1) - z.amin(-1)).clamp(max=1e30) + math.log(vocab)
+    lp_tol = rel.squeeze(-1) + 8 * U * size
+    grad_tol = half_step(grad, dtype) * 1.01 + g.abs() * (p * rel + 4 * U * (p + grad.abs() / g.abs().clamp(min=1e-30)))
+    return lp_tol, grad_tol
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 7), (4, 8), (2, 503), (3, 4097), (2, 50257), (1030, 2049)])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_log_probs_and_gradient(device, dtype, shape, temperature):
+    rows, vocab = shape
+    g = gen(rows + vocab)
+    logits = (torch.randn(rows, vocab, generator=g) * 4).to(dtype).to(device).requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    if rows > 2:
+        tokens[1] = -100
+    tokens = tokens.to(device)
+    upstream = torch.randn(rows, generator=g).to(device)
+    lp = ops.token_log_probs(logits, tokens, temperature=temperature)
+    assert lp.dtype == torch.float32
+    (grad,) = torch.autograd.grad(lp, logits, upstream)
+    assert grad.dtype == dtype
+    want, dwant, gg, p, z = log_probs_oracle(logits, tokens, temperature, -100, upstream)
+    lp_tol, grad_tol = log_probs_tolerance(z, gg, p, dwant, vocab, dtype)
+    close(lp, want, lp_tol)
+    close(grad, dwant, grad_tol)
+    with torch.no_grad():
+        assert torch.equal(ops.token_log_probs(logits, tokens, temperature=temperature), lp)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_strided_rows(device, dtype):
+    """The rows that predict a response, inside the logits of the whole
+    sequence; int32 tokens; four leading dims; a transposed layout."""
+    g = gen(3)
+    whole = torch.randn(3, 9, 131, generator=g).to(dtype).to(device).requires_grad_()
+    tokens = torch.randint(0, 131, (3, 4), generator=g).to(device)
+    upstream = torch.randn(3, 4, generator=g).to(device)
+    lp = ops.token_log_probs(whole[:, 4:8], tokens.int())
+    (grad,) = torch.autograd.grad(lp, whole, upstream)
+    want, dwant, gg, p, z = log_probs_oracle(whole[:, 4:8], tokens, 1.0, -100, upstream)
+    lp_tol, grad_tol = log_probs_tolerance(z, gg, p, dwant, 131, dtype)
+    close(lp, want, lp_tol)
+    close(grad[:, 4:8], dwant, grad_tol)
+    assert (grad[:, :4] == 0).all() and (grad[:, 8:] == 0).all()
+    turned = whole[:, 4:8].detach().transpose(1, 2).contiguous().transpose(1, 2)
+    assert turned.stride(-1) != 1
+    close(ops.token_log_probs(turned, tokens), want, lp_tol)
+    many = whole[:, 4:8].detach().reshape(3, 2, 2, 131)[None]
+    got = ops.token_log_probs(many, tokens.reshape(1, 3, 2, 2))
+    close(got.reshape(3, 4), want, lp_tol)
+    single = ops.token_log_probs(whole[0, 4].detach(), tokens[0, 0])
+    close(single, want[0, 0], lp_tol[0, 0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [70, 3001])
+def test_log_probs_masked_vocabulary(device, dtype, vocab):
+    """-inf and the lowest value in masked columns, rows of nothing else, NaN
+    in ignored rows and under a zero upstream gradient."""
+    g = gen(vocab)
+    low = torch.finfo(dtype).min
+    logits = torch.randn(7, vocab, generator=g)
+    logits[0, vocab // 2:] = -math.inf
+    logits[1, : vocab // 3] = low
+    logits[2] = low                   # uniform
+    logits[3] = -math.inf             # no distribution: NaN
+    logits[4] = math.nan              # ignored
+    logits[5] = math.nan              # its upstream gradient is 0
+    logits = logits.to(dtype).to(device).requires_grad_()
+    tokens = torch.tensor([1, vocab - 1, 3, 0, -100, 2, 5], device=device)
+    upstream = torch.tensor([1.0, -2.0, 0.5, 1.0, 1.0, 0.0, 3.0], device=device)
+    lp = ops.token_log_probs(logits, tokens)
+    got = lp.detach().cpu().double()
+    assert got[3].isnan() and got[5].isnan() and got[4] == 0
+    assert abs(got[2] + math.log(vocab)) < 64 * U * math.log(vocab)
+    rest = [0, 1, 6]
+    want, dwant, gg, p, z = log_probs_oracle(logits[rest], tokens[rest], 1.0, -100, upstream[rest])
+    close(lp[rest], want, U * (6 * 40 + vocab / 64 + 64))
+    if device == "cpu":
+        return  # log_softmax's own backward knows no masked rows
+    (grad,) = torch.autograd.grad(lp, logits, upstream)
+    grad = grad.cpu()
+    assert (grad[4] == 0).all() and (grad[5] == 0).all()
+    assert grad[3].isnan().all()
+    close(grad[rest], dwant, half_step(dwant, dtype) * 1.01 + gg.abs() * U * (6 * 40 + vocab / 64 + 64))
+    uniform = torch.full((vocab,), -0.5 / vocab, dtype=torch.float64)
+    uniform[3] += 0.5
+    close(grad[2], uniform, half_step(uniform, dtype) * 1.01 + U * 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_tokens_out_of_range(device):
+    logits = torch.randn(4, 9, generator=gen(0)).to(device)
+    tokens = torch.tensor([-1, 9, 2 ** 40, 3], device=device)
+    lp = ops.token_log_probs(logits, tokens)
+    assert lp[:3].isnan().all() and lp[3].isfinite()
+    lp = ops.token_log_probs(logits, tokens, ignore_index=-1)
+    assert lp[0] == 0 and lp[1:3].isnan().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_empty(device):
+    logits = torch.zeros(0, 5, 7, device=device, requires_grad=True)
+    lp = ops.token_log_probs(logits, torch.zeros(0, 5, dtype=torch.long, device=device))
+    assert lp.shape == (0, 5)
+    (grad,) = torch.autograd.grad(lp.sum(), logits)
+    assert grad.shape == logits.shape
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_gradient_against_differences(device):
+    """Central differences of step h in float32: the third derivative (below 1
+    in softmax) leaves h^2 / 6, the rounding of lp leaves 2 * 16 u |lp| / h."""
+    g = gen(9)
+    logits = torch.randn(3, 12, generator=g).to(device).requires_grad_()
+    tokens = torch.tensor([0, 5, 11], device=device)
+    (grad,) = torch.autograd.grad(ops.token_log_probs(logits, tokens, temperature=0.8).sum(), logits)
+    h = 2.0 ** -7
+    for i in range(3):
+        for j in range(12):
+            up, down = logits.detach().clone(), logits.detach().clone()
+            up[i, j] += h
+            down[i, j] -= h
+            d = (ops.token_log_probs(up, tokens, temperature=0.8)[i]
+                 - ops.token_log_probs(down, tokens, temperature=0.8)[i]) / (2 * h)
+            assert abs(float(d - grad[i, j])) < h * h / 6 / 0.8 ** 3 + 32 * U * 10 / h
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_refusals(device):
+    logits = torch.zeros(2, 5, device=device)
+    tokens = torch.zeros(2, dtype=torch.long, device=device)
+    with pytest.raises(TypeError, match="logits must be"):
+        ops.token_log_probs(logits.double(), tokens)
+    with pytest.raises(TypeError, match="tokens must be"):
+        ops.token_log_probs(logits, tokens.float())
+    with pytest.raises(ValueError, match="shape of logits"):
+        ops.token_log_probs(logits, tokens[:1])
+    with pytest.raises(ValueError, match="vocabulary"):
+        ops.token_log_probs(logits[:, :0], tokens)
+    for bad in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_log_probs(logits, tokens, temperature=bad)
+    if device == "cuda":
+        with pytest.raises(ValueError, match="tokens is on"):
+            ops.token_log_probs(logits, tokens.cpu())
+        leaf = logits.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(ops.token_log_probs(leaf, tokens).sum(), leaf, create_graph=True)
+
+
+# --------------------------------------------------------------------------- #
+# token_policy_loss
+# --------------------------------------------------------------------------- #
+def policy_oracle(lp, old, adv, w, ref, low, high, variant, kl_c, ent_c, reduction):
+    lp = lp.detach().cpu().double().requires_grad_()
+    old = old.cpu().double()
+    adv = adv.cpu().double().expand(lp.shape)
+    w = torch.ones_like(lp) if w is None else w.cpu().double()
+    keep = w != 0
+    x = (lp - old)[keep]
+    r = x.exp()
+    c = r.clamp(1 - low, 1 + high)
+    a, ww = adv[keep], w[keep]
+    gain = torch.minimum(r * a, c * a) if variant == "clip" else c.detach() * x * a
+    count = max(1.0, float(w.sum())) if reduction == "mean" else 1.0
+    obj = -(gain * ww).sum() / count
+    kl = torch.zeros((), dtype=torch.float64)
+    ysize = kl
+    if ref is not None:
+        y = (ref.cpu().double() - lp)[keep]
+        kl = ((y.expm1() - y) * ww).sum() / count
+        ysize = ((y.exp() + 1 + y.abs()) * ww.abs()).detach()
+    ent = ent_c * (lp[keep] * ww).sum() / count
+    total = obj + kl_c * kl + ent
+    (grad,) = torch.autograd.grad(total, lp)
+    every = (lp.detach() - old).exp()
+    out = dict(loss_total=total, loss_objective=obj, loss_kl=kl_c * kl, loss_entropy=ent, kl=kl,
+               clip_fraction=((every - 1).abs() > low).double().mean(),
+               ess=every.sum() ** 2 / (every ** 2).sum().clamp(min=1e-9) / every.numel(), grad=grad)
+    size = dict(gain=float((gain * ww).detach().abs().sum() / count),
+                kl=float(ysize.sum() / count) if ref is not None else 0.0,
+                x=float(x.detach().abs().max()) if x.numel() else 0.0)
+    # what a gradient's terms come to, one by one
+    terms = torch.zeros_like(lp.detach())
+    terms[keep] = (r * a).abs().detach() + (c * a).abs().detach() + abs(ent_c)
+    if ref is not None:
+        terms[keep] += abs(kl_c) * ysize / ww.abs()
+    return {k: v.detach() for k, v in out.items()}, size, terms * w.abs() / count
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 5), (16, 45), (1, 4099), (130, 257)])
+@pytest.mark.parametrize("variant,high,kl,ent,reduction,masked", [
+    ("clip", 0.2, 0.0, 0.0, "mean", "bool"),
+    ("clip", 0.28, 0.05, 0.01, "mean", "int64"),
+    ("cispo", 0.2, 0.02, 0.0, "sum", "float"),
+    ("clip", 0.2, 0.1, 0.0, "sum", None),
+])
+def test_policy_loss_and_gradient(device, dtype, shape, variant, high, kl, ent, reduction, masked):
+    g = gen(shape[1])
+    old = (-torch.randn(shape, generator=g).abs() * 2).to(dtype)
+    lp = (old.float() + 0.3 * torch.randn(shape, generator=g)).to(dtype)
+    ref = (old.float() + 0.3 * torch.randn(shape, generator=g)).to(dtype) if kl else None
+    adv = torch.randn(shape[0], 1, generator=g)
+    mask = None
+    if masked:
+        mask = torch.rand(shape, generator=g) < 0.7
+        if masked == "int64":
+            mask = mask.long()
+        elif masked == "float":
+            mask = mask * torch.rand(shape, generator=g)
+    move = lambda t: None if t is None else t.to(device)  # noqa: E731
+    leaf = lp.to(device).requires_grad_()
+    out = ops.token_policy_loss(
+        leaf, move(old), move(adv), move(mask), move(ref), clip_low=0.2, clip_high=high,
+        variant=variant, kl_coeff=kl, entropy_coeff=ent, reduction=reduction)
+    (grad,) = torch.autograd.grad(out.loss_total, leaf)
+    want, size, terms = policy_oracle(lp, old, adv, mask, ref, 0.2, high, variant, kl, ent, reduction)
+    # an element is off by u |x| through its exponent and by a few roundings;
+    # a sum in float32 (the CPU form) rounds log2(n) times on the way
+    n = lp.numel()
+    step = U * (8 + 2 * size["x"] + (0 if device == "cuda" else 2 * math.log2(n + 1) + 8))
+    lp_mean = float((lp.detach().double().abs() * (1 if mask is None else mask.double().abs())).sum()) / (
+        1.0 if reduction == "sum" else max(1.0, float(n if mask is None else mask.sum())))
+    near = dict(loss_objective=step * size["gain"], kl=step * size["kl"],
+                loss_entropy=step * abs(ent) * lp_mean, clip_fraction=U, ess=4 * step)
+    near["loss_kl"] = kl * near["kl"]
+    near["loss_total"] = near["loss_objective"] + near["loss_kl"] + near["loss_entropy"]
+    for name, tol in near.items():
+        got = float(getattr(out, name).detach())
+        ref_v = float(want[name])
+        assert abs(got - ref_v) <= 2 * tol + 2 * U * abs(ref_v), (name, got, ref_v)
+    close(grad, want["grad"], 1.01 * half_step(want["grad"], dtype) + 2 * step * terms)
+    with torch.no_grad():
+        again = ops.token_policy_loss(
+            leaf, move(old), move(adv), move(mask), move(ref), clip_low=0.2, clip_high=high,
+            variant=variant, kl_coeff=kl, entropy_coeff=ent, reduction=reduction)
+    assert all(torch.equal(a, b) for a, b in zip(again, out))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_loss_separate_gradients_and_layouts(device):
+    """Each differentiable output by itself; strided and mixed-type operands;
+    more than two dims."""
+    g = gen(5)
+    wide = torch.randn(2, 3, 2 * 10, generator=g)
+    lp = (-wide[..., ::2].abs()).to(device)
+    old = (lp.cpu() + 0.2 * torch.randn(2, 3, 10, generator=g)).bfloat16().to(device)
+    ref = (lp.cpu() + 0.2 * torch.randn(3, 2, 10, generator=g).transpose(0, 1)).to(device)
+    adv = torch.randn(3, 1, generator=g).to(device)
+    mask = (torch.rand(10, 3, 2, generator=g) < 0.6).permute(2, 1, 0).to(device)
+    for pick in ("loss_objective", "loss_kl", "loss_entropy"):
+        leaf = lp.clone().requires_grad_()
+        out = ops.token_policy_loss(leaf, old, adv, mask, ref, kl_coeff=0.1, entropy_coeff=0.3)
+        (grad,) = torch.autograd.grad(3.0 * getattr(out, pick), leaf)
+        ref_leaf = lp.double().cpu().requires_grad_()
+        x = ref_leaf - old.double().cpu()
+        r = x.exp()
+        a = adv.double().cpu()
+        y = ref.double().cpu() - ref_leaf
+        term = {"loss_objective": -torch.minimum(r * a, r.clamp(0.8, 1.2) * a),
+                "loss_kl": 0.1 * (y.expm1() - y), "loss_entropy": 0.3 * ref_leaf}[pick]
+        keep = mask.cpu()
+        (want,) = torch.autograd.grad(3.0 * term[keep].sum() / keep.sum(), ref_leaf)
+        close(grad, want, 64 * U * (want.abs() + 3.0 / float(keep.sum())))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_loss_masked_places_hold_anything(device):
+    lp = torch.tensor([[-1.0, math.nan, -2.0, math.inf]], device=device, requires_grad=True)
+    old = torch.tensor([[-1.1, -math.inf, -2.0, math.nan]], device=device)
+    ref = torch.tensor([[-0.9, math.nan, -2.5, -math.inf]], device=device)
+    mask = torch.tensor([[True, False, True, False]], device=device)
+    out = ops.token_policy_loss(lp, old, torch.ones(1, 1, device=device), mask, ref, kl_coeff=0.1)
+    (grad,) = torch.autograd.grad(out.loss_total, lp)
+    assert out.loss_total.isfinite() and grad.isfinite().all()
+    assert grad[0, 1] == 0 and grad[0, 3] == 0 and (grad[0, ::2] != 0).all()
+    nothing = ops.token_policy_loss(lp, old, torch.ones(1, 1, device=device),
+                                    torch.zeros_like(mask), ref, kl_coeff=0.1)
+    assert nothing.loss_total == 0 and nothing.kl == 0
+    (grad,) = torch.autograd.grad(nothing.loss_total, lp)
+    assert (grad == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_loss_outputs_change_in_place(device):
+    lp = torch.zeros(2, 3, device=device, requires_grad=True)
+    out = ops.token_policy_loss(lp, torch.zeros(2, 3, device=device), torch.ones(2, 1, device=device))
+    total = out.loss_total
+    kept = float(out.loss_objective.detach())
+    total += 1.0
+    assert float(out.loss_objective.detach()) == kept
+    total.backward()
+    assert torch.allclose(lp.grad, torch.full_like(lp, -1 / 6))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_loss_refusals(device):
+    lp = torch.zeros(2, 3, device=device)
+    adv = torch.zeros(2, 1, device=device)
+
+    def call(a=lp, b=lp, c=adv, **kw):
+        return ops.token_policy_loss(a, b, c, kw.pop("mask", None), kw.pop("ref", None), **kw)
+
+    with pytest.raises(TypeError, match="log_probs must be"):
+        call(a=lp.double(), b=lp)
+    with pytest.raises(ValueError, match="old_log_probs must have"):
+        call(b=lp[:1])
+    with pytest.raises(ValueError, match="does not broadcast"):
+        call(c=torch.zeros(3, 1, device=device))
+    with pytest.raises(ValueError, match="mask must have"):
+        call(mask=torch.ones(2, device=device))
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        call(mask=torch.ones(2, 3, dtype=torch.complex64, device=device))
+    with pytest.raises(ValueError, match="must not require"):
+        call(b=lp.clone().requires_grad_())
+    with pytest.raises(ValueError, match="must not require"):
+        call(c=adv.clone().requires_grad_())
+    with pytest.raises(ValueError, match="empty"):
+        call(a=lp[:, :0], b=lp[:, :0])
+    with pytest.raises(ValueError, match="clip_low"):
+        call(clip_low=-0.1)
+    with pytest.raises(ValueError, match="coeff"):
+        call(kl_coeff=math.nan)
+    with pytest.raises(ValueError, match="variant"):
+        call(variant="ppo")
+    with pytest.raises(ValueError, match="reduction"):
+        call(reduction="none")
+    if device == "cuda":
+        leaf = lp.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(call(a=leaf).loss_total, leaf, create_graph=True)
+
+
+# --------------------------------------------------------------------------- #
+# the paged cache
+# --------------------------------------------------------------------------- #
+def make_cache(g, batch, columns, kv_heads, page, dim, dtype, device, spare=2):
+    """A cache whose free pages and slots hold NaN, and a shuffled table."""
+    pages = batch * columns + spare
+    k = torch.full((pages, kv_heads, page, dim), math.nan)
+    table = torch.randperm(pages, generator=g)[: batch * columns].reshape(batch, columns).int()
+    return k.to(dtype).to(device), k.clone().to(dtype).to(device), table.to(device)
+
+
+def rotate64(x, cos, sin, interleaved):
+    """[T, H, D] by [T, R / 2] as complex numbers."""
+    half = cos.shape[-1]
+    one = slice(0, 2 * half, 2) if interleaved else slice(0, half)
+    two = slice(1, 2 * half, 2) if interleaved else slice(half, 2 * half)
+    y = x.clone()
+    z = torch.complex(x[..., one], x[..., two]) * torch.complex(cos, sin).unsqueeze(1)
+    y[..., one], y[..., two] = z.real, z.imag
+    return y
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,width,heads,kv_heads,dim,page,rotary,interleaved,odd", [
+    (3, 1, 4, 4, 64, 16, 0, False, False),
+    (3, 1, 8, 2, 128, 8, 128, False, False),
+    (2, 7, 12, 4, 80, 4, 80, True, False),
+    (2, 19, 5, 1, 96, 16, 48, False, False),
+    (4, 5, 6, 3, 80, 1, 40, False, False),
+    (2, 33, 16, 2, 256, 32, 256, True, False),
+    (3, 6, 3, 3, 40, 8, 20, True, True),
+    (3, 6, 2, 1, 8, 64, 8, False, True),
+    (1, 3, 40, 40, 64, 16, 2, False, False),
+])
+def test_append(device, dtype, batch, width, heads, kv_heads, dim, page, rotary, interleaved, odd):
+    g = gen(dim + width)
+    past = 11
+    columns = -(-(past + width) // page)
+    k_cache, v_cache, table = make_cache(g, batch, columns, kv_heads, page, dim, dtype, device)
+    # views of one projection; `odd` shifts them off every alignment
+    rows = torch.randn(batch, width, (heads + 2 * kv_heads) * dim + 1, generator=g).to(dtype).to(device)
+    rows = rows[..., 1:] if odd else rows[..., :-1].contiguous()
+    q, k, v = rows.split([heads * dim, kv_heads * dim, kv_heads * dim], -1)
+    q, k, v = (t.unflatten(-1, (-1, dim)) for t in (q, k, v))
+    start = torch.randint(0, past, (batch,), generator=g)
+    lengths = torch.randint(0, width + 1, (batch,), generator=g)
+    lengths[0] = width
+    if batch > 2:
+        lengths[1] = 0
+    rope = ops.rotary_table(past + width, rotary, device=device) if rotary else None
+    got_q = ops.paged_kv_append(
+        k, v, k_cache, v_cache, table, start.to(device).int(), lengths=lengths.to(device),
+        q=q if rotary else None, rope=rope, interleaved=interleaved)
+    assert (got_q is None) == (rotary == 0)
+    want_k = torch.full(k_cache.shape, math.nan, dtype=torch.float64)
+    want_v, size = want_k.clone(), want_k.clone()
+    want_q = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(batch):
+        n, first = int(lengths[b]), int(start[b])
+        kk, qq = k[b, :n].cpu().double(), q[b, :n].cpu().double()
+        if rotary:
+            cos, sin = (t[first:first + n].cpu().double() for t in rope)
+            kk, qq = (rotate64(t, cos, sin, interleaved) for t in (kk, qq))
+            want_q[b, :n] = qq
+        place = torch.arange(first, first + n)
+        at = table[b].cpu().long()[place // page]
+        want_k[at, :, place % page] = kk
+        want_v[at, :, place % page] = v[b, :n].cpu().double()
+    # two products and a sum in float32, each rounded, then the cache's rounding
+    worst = float(rows.abs().max()) * 4 * U
+    close(v_cache, want_v, 0.0)
+    close(k_cache, want_k, 1.01 * half_step(want_k, dtype) + worst if rotary else 0.0)
+    if rotary:
+        close(got_q, want_q, 1.01 * half_step(want_q, dtype) + worst)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_append_bad_places_write_nothing(device):
+    g = gen(1)
+    k_cache, v_cache, _ = make_cache(g, 6, 1, 2, 8, 16, torch.float32, device)
+    before = k_cache.clone()
+    table = torch.tensor([[-1], [8], [2 ** 31 - 1], [2], [3], [4]], dtype=torch.int32, device=device)
+    assert k_cache.shape[0] == 8
+    start = torch.tensor([0, 0, 0, -2, 7, 2 ** 33], device=device)
+    k = torch.randn(6, 2, 2, 16, generator=g).to(device)
+    ops.paged_kv_append(k, k, k_cache, v_cache, table, start)
+    before[3, :, 7] = k[4, 0]
+    assert torch.equal(k_cache.isnan(), before.isnan())
+    assert torch.equal(k_cache.nan_to_num(), before.nan_to_num())
+    empty = torch.zeros(6, 0, dtype=torch.int32, device=device)
+    ops.paged_kv_append(k, k, k_cache, v_cache, empty, start)
+    ops.paged_kv_append(k[:0], k[:0], k_cache, v_cache, table[:0], start[:0])
+    ops.paged_kv_append(k[:, :0], k[:, :0], k_cache, v_cache, table, start)
+    assert torch.equal(k_cache.nan_to_num(), before.nan_to_num())
+    # past the rotation's table: NaN, not what lies behind it
+    rope = ops.rotary_table(3, 16, device=device)
+    zero = torch.zeros(6, dtype=torch.int32, device=device)
+    good = torch.arange(6, dtype=torch.int32, device=device)[:, None]
+    wide = k.repeat(1, 2, 1, 1)
+    q = ops.paged_kv_append(wide, wide, k_cache, v_cache, good, zero, q=wide, rope=rope)
+    assert q[:, :3].isfinite().all() and q[:, 3].isnan().all()
+    assert k_cache[:6, :, :3].isfinite().all() and k_cache[:6, :, 3].isnan().all()
+
+
+def attend_oracle(q, k_cache, v_cache, table, lengths, scale):
+    q, k_cache, v_cache = (t.cpu().double() for t in (q, k_cache, v_cache))
+    table = table.cpu().long()
+    batch, heads, dim = q.shape
+    kv_heads, page = k_cache.shape[1:3]
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for b in range(batch):
+        n = min(int(lengths[b]), table.shape[1] * page)
+        place = torch.arange(max(0, n))
+        at = table[b][place // page] if n > 0 else place
+        keep = (at >= 0) & (at < k_cache.shape[0])
+        place, at = place[keep], at[keep]
+        if not len(place):
+            continue
+        for h in range(heads):
+            kv = h // (heads // kv_heads)
+            k, v = k_cache[at, kv, place % page], v_cache[at, kv, place % page]
+            score = (k @ q[b, h]) * scale
+            p = torch.softmax(score, 0)
+            out[b, h] = p @ v
+            # a score of dim products adds up in float32 (the matrix unit may cut
+            # instead of rounding: 2 u each); exp turns its error into a relative
+            # one; weights enter the second product in two 16-bit parts (2^-16);
+            # the sums over n keys round n times at most
+            off = float(((k.abs() @ q[b, h].abs()) * abs(scale)).max()) * 2 * U * (dim + 8)
+            rel = 2 * off + 2.0 ** -16 + 2 * U * (len(place) + 16)
+            tol[b, h] = rel * (p @ v.abs())
+    return out, tol
+
+
+def fill_cache(g, cache, table, lengths):
+    """Random keys or values in the slots that sequences hold; NaN elsewhere."""
+    page = cache.shape[2]
+    for b in range(table.shape[0]):
+        n = min(int(lengths[b]), table.shape[1] * page)
+        if n <= 0:
+            continue
+        place = torch.arange(n)
+        at = table[b].cpu().long()[place // page]
+        cache[at, :, place % page] = torch.randn(n, cache.shape[1], cache.shape[3], generator=g).to(
+            cache.dtype).to(cache.device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [
+    ([1], 1, 1, 64, 16),
+    ([0, 1, 2, 17], 4, 4, 64, 16),
+    ([31, 32, 33, 64, 65], 8, 2, 128, 8),
+    ([100, 7], 14, 2, 80, 4),
+    ([257, 0, 300], 12, 12, 64, 16),
+    ([1000], 5, 1, 96, 1),
+    ([511, 513, 129], 32, 2, 256, 128),
+    ([77, 40], 40, 1, 40, 32),
+    ([33], 16, 16, 8, 2),
+    ([5000, 3, 129, 2048], 32, 8, 128, 64),
+    ([3000] * 3, 7, 1, 192, 256),
+    ([-3, 9], 24, 1, 64, 16),
+])
+def test_attend(device, dtype, lengths, heads, kv_heads, dim, page):
+    g = gen(sum(lengths) + dim)
+    batch = len(lengths)
+    columns = max(1, -(-max(lengths) // page))
+    k_cache, v_cache, table = make_cache(g, batch, columns, kv_heads, page, dim, dtype, device)
+    fill_cache(g, k_cache, table, lengths)
+    fill_cache(g, v_cache, table, lengths)
+    q = (torch.randn(batch, heads, dim, generator=g) * 2).to(dtype).to(device)
+    count = torch.tensor(lengths, device=device)
+    out = ops.paged_attention_decode(q, k_cache, v_cache, table, count)
+    assert out.dtype == dtype and out.is_contiguous()
+    want, tol = attend_oracle(q, k_cache, v_cache, table, lengths, dim ** -0.5)
+    close(out, want, 1.01 * half_step(want, dtype) + tol)
+    again = ops.paged_attention_decode(q, k_cache, v_cache, table, count.int(), scale=dim ** -0.5)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attend_bad_pages_and_layouts(device, dtype):
+    """Missing pages are left out, a length past the table is cut, layer views
+    of a bigger cache and strided queries and tables are read in place."""
+    g = gen(8)
+    batch, heads, kv_heads, dim, page, columns = 4, 6, 3, 64, 16, 5
+    k_cache, v_cache, table = make_cache(g, batch, columns, kv_heads, page, dim, dtype, device)
+    lengths = [columns * page] * batch
+    fill_cache(g, k_cache, table, lengths)
+    fill_cache(g, v_cache, table, lengths)
+    layers_k, layers_v = (torch.full((2,) + t.shape[:2] + (3,) + t.shape[2:], math.nan, dtype=dtype, device=device)
+                          for t in (k_cache, v_cache))
+    layers_k[1, :, :, 2] = k_cache
+    layers_v[1, :, :, 2] = v_cache
+    wide = torch.full((batch, 2 * columns), 2 ** 30, dtype=torch.int32, device=device)
+    wide[:, ::2] = table
+    table = wide[:, ::2]
+    table[0, 1], table[0, 4], table[1, 0] = -1, k_cache.shape[0], 2 ** 31 - 1
+    table[2] = -5
+    lengths = [79, 10, 80, 10 ** 9]
+    q = torch.randn(batch, 2 * heads, dim + 8, generator=g).to(dtype).to(device)[:, ::2, :dim]
+    out = ops.paged_attention_decode(
+        q, layers_k[1, :, :, 2], layers_v[1, :, :, 2], table, torch.tensor(lengths, device=device), scale=0.3)
+    want, tol = attend_oracle(q, k_cache, v_cache, table, lengths, 0.3)
+    assert (want[1] == 0).all() and (want[2] == 0).all()
+    close(out, want, 1.01 * half_step(want, dtype) + tol)
+    odd = torch.randn(batch, heads, dim + 1, generator=g).to(dtype).to(device)[..., 1:]
+    out = ops.paged_attention_decode(odd, k_cache, v_cache, table, torch.tensor(lengths, device=device))
+    want, tol = attend_oracle(odd, k_cache, v_cache, table, lengths, dim ** -0.5)
+    close(out, want, 1.01 * half_step(want, dtype) + tol)
+    none = ops.paged_attention_decode(q, k_cache, v_cache, table[:, :0], torch.tensor(lengths, device=device))
+    assert (none == 0).all()
+    assert ops.paged_attention_decode(
+        q[:0], k_cache, v_cache, table[:0], torch.zeros(0, dtype=torch.int32, device=device)).shape == (0, heads, dim)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attend_one_key_dominates(device, dtype):
+    """A score far above the rest, first, last or in the middle, gives that
+    key's value: the others' weights are below exp(-60)."""
+    g = gen(2)
+    n, dim, page = 700, 64, 16
+    for hot in (0, 350, 699):
+        k_cache, v_cache, table = make_cache(g, 1, 44, 1, page, dim, dtype, device)
+        fill_cache(g, k_cache, table, [n])
+        fill_cache(g, v_cache, table, [n])
+        at = int(table[0, hot // page])
+        k_cache[at, 0, hot % page] = 16.0
+        q = torch.full((1, 2, dim), 1.0, dtype=dtype, device=device)
+        out = ops.paged_attention_decode(q, k_cache, v_cache, table, torch.tensor([n], device=device))
+        assert torch.equal(out[0, 0], v_cache[at, 0, hot % page])
+        assert torch.equal(out[0, 1], out[0, 0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_paged_refusals(device):
+    k_cache = torch.zeros(4, 2, 8, 16, device=device)
+    v_cache = torch.zeros_like(k_cache)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=device)
+    start = torch.zeros(3, dtype=torch.int32, device=device)
+    k = torch.zeros(3, 1, 2, 16, device=device)
+    q4, q = torch.zeros(3, 1, 4, 16, device=device), torch.zeros(3, 4, 16, device=device)
+    rope = ops.rotary_table(8, 16, device=device)
+
+    def append(k=k, v=None, kc=k_cache, vc=v_cache, t=table, s=start, **kw):
+        return ops.paged_kv_append(k, k if v is None else v, kc, vc, t, s, **kw)
+
+    def attend(q=q, kc=k_cache, vc=v_cache, t=table, n=start, **kw):
+        return ops.paged_attention_decode(q, kc, vc, t, n, **kw)
+
+    for bad, error, text in [
+        (dict(k=k[0]), ValueError, "k and v must be"),
+        (dict(v=k[:, :, :1]), ValueError, "k and v must be"),
+        (dict(k=k.bfloat16()), TypeError, "cache's dtype"),
+        (dict(kc=k_cache.double(), vc=v_cache.double()), TypeError, "share one dtype"),
+        (dict(vc=v_cache.half()), TypeError, "share one dtype"),
+        (dict(kc=k_cache[:, :, :6], vc=v_cache[:, :, :6]), ValueError, "power of two"),
+        (dict(kc=k_cache[:, :1], vc=v_cache[:, :1]), ValueError, "expected 2 of"),
+        (dict(kc=k_cache[:0], vc=v_cache[:0]), ValueError, "pages"),
+        (dict(kc=k_cache.transpose(2, 3).contiguous().transpose(2, 3)), ValueError, "dense"),
+        (dict(t=table.long()), TypeError, "page_table must be int32"),
+        (dict(t=table[:2]), ValueError, "page_table must be"),
+        (dict(s=start[:2]), ValueError, "start must be"),
+        (dict(s=start.float()), TypeError, "start must be"),
+        (dict(lengths=start[:2]), ValueError, "lengths must be"),
+        (dict(q=q4), ValueError, "no rope"),
+        (dict(q=q, rope=rope), ValueError, "q must be"),
+        (dict(q=q4.half(), rope=rope), TypeError, "q must have"),
+        (dict(rope=(rope[0].double(), rope[1].double())), TypeError, "rope must be float32"),
+        (dict(rope=(rope[0], rope[1][:4])), ValueError, "rope must be"),
+        (dict(rope=(rope[0].repeat(1, 2), rope[1].repeat(1, 2))), ValueError, "rope must be"),
+        (dict(rope=(rope[0][:, ::2], rope[1][:, ::2])), ValueError, "contiguous"),
+        (dict(k=k.clone().requires_grad_()), ValueError, "no_grad"),
+    ]:
+        with pytest.raises(error, match=text):
+            append(**bad)
+    shifted = torch.zeros(4 * 2 * 8 * 16 + 1, device=device)[1:].view(4, 2, 8, 16)
+    for bad, error, text in [
+        (dict(q=q[0]), ValueError, "q must be"),
+        (dict(q=q[:, :3]), ValueError, "divisor"),
+        (dict(q=q.half()), TypeError, "cache's dtype"),
+        (dict(q=q[:, :, :8]), ValueError, "expected 2 of"),
+        (dict(kc=shifted), ValueError, "aligned"),
+        (dict(n=start[:1]), ValueError, "lengths must be"),
+        (dict(t=table[0]), ValueError, "page_table must be"),
+        (dict(scale=math.inf), ValueError, "scale"),
+        (dict(q=q.clone().requires_grad_()), ValueError, "no_grad"),
+    ]:
+        with pytest.raises(error, match=text):
+            attend(**bad)
+    small = torch.zeros(4, 2, 8, 12, device=device)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        attend(q=q[:, :, :12], kc=small, vc=small)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        ops.rotary_table(4, 3)
+    with torch.no_grad():
+        assert append(k=k.clone().requires_grad_()) is None
+    if device == "cuda":
+        with pytest.raises(ValueError, match="is on"):
+            attend(n=start.cpu())
