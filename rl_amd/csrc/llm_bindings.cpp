@@ -157,7 +157,9 @@ void cache_check(const char* op, const Tensor& k_cache, const Tensor& v_cache,
   TORCH_CHECK_VALUE(page_table.dim() == 2 && page_table.size(0) == batch, op,
                     ": page_table must be [batch, pages] with batch ", batch, ", got ",
                     page_table.sizes());
-  TORCH_CHECK_VALUE(page_table.size(1) <= INT32_MAX / page, op, ": page_table has too many columns");
+  TORCH_CHECK_VALUE(page_table.size(1) <= (int64_t(1) << 30) / page, op,
+                    ": page_table must span at most 2**30 positions, got ", page_table.size(1),
+                    " pages of ", page);
 }
 
 void per_sequence(const char* op, const Tensor& t, const char* name, int64_t batch,
@@ -607,7 +609,16 @@ Tensor paged_attention_decode(const Tensor& q_in, const Tensor& k_cache, const T
   a.dim = (int)q.size(2);
   a.dtype = code_of(q, "paged_attention_decode");
   a.scale = (float)(scale * 1.4426950408889634);
-  if (a.batch) launched(launch_paged_attend(&a, stream_of()), "paged_attention_decode");
+  if (!a.batch) return out;
+  plan_paged_attend(&a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  Tensor part;
+  if (a.workers) {
+    const int64_t rows = 2 * (int64_t)a.workers * std::min(16, a.heads / a.kv_heads);
+    part = torch::empty({rows * (a.dim + 2)}, q.options().dtype(torch::kFloat32));
+    a.part = part.data_ptr<float>();
+    a.part_ms = a.part + rows * a.dim;
+  }
+  launched(launch_paged_attend(&a, stream_of()), "paged_attention_decode");
   return out;
 }
 

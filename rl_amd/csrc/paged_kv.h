@@ -46,9 +46,17 @@ struct PagedAttendArgs {
   int heads, kv_heads, dim;
   int dtype;
   float scale;             // of the scores, times log2(e)
+  // the plan: filled in by plan_paged_attend
+  int head_blocks;         // blocks of 16 query heads per key head
+  int workers;             // 0: one workgroup per (sequence, key head, block)
+  int waves;               // of a workgroup
+  // workspace where workers > 0
+  float* part;             // [2 * workers][min(16, heads / kv_heads)][dim]
+  float* part_ms;          // [2 * workers][min(16, heads / kv_heads)][2]
 };
 
 extern "C" {
 int launch_paged_append(const PagedAppendArgs* a, void* stream);
+void plan_paged_attend(PagedAttendArgs* a, int cus);
 int launch_paged_attend(const PagedAttendArgs* a, void* stream);
 }

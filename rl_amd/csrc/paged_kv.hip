@@ -201,78 +201,672 @@ int append_vec(const PagedAppendArgs& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// paged_attend, the simple form: one workgroup per (sequence, head), its four
-// waves over every fourth key, 64 lanes over the dims, the running maximum and
-// sum of the softmax in fp32, and one join at the end.
+// paged_attend: out = softmax(scale q k^T) v for one query token per sequence.
+//
+// The G = heads / kv_heads query heads that share a key head are the 16 columns
+// of one matrix tile (padded; more than 16 take ceil(G / 16) blocks).  Both
+// products are turned so that a lane keeps one query head throughout:
+//
+//   S^T [keys x heads] = K Q^T     A = K: lane l holds 16 bytes of key row l % 16,
+//                                  straight from the cache, no shared memory
+//   O^T [dims x heads] = V^T P^T   B = P: what the first product and the softmax
+//                                  left in the lane's registers is its operand
+//                                  (the order of the keys within a product is
+//                                  free); A = V^T comes through shared memory
+//                                  with a transposing read
+//
+// so the running maximum, the sum and the rescaling of the output are per lane,
+// and a tile of keys costs two shuffles.  Weights enter the second product as
+// two 16-bit parts (the rounded weight and what it left), so that they are not
+// rounded to 8 bits for bfloat16; the matrix unit has the time, the kernel is
+// bound by the cache's bytes.  float32 caches use the fp32 matrix instruction on
+// tiles of 16 keys, with V's operand read directly.
+//
+// A wave owns whole tiles: while it computes one, the keys, values and page ids
+// of the next are on their way in its registers.  No barrier in the loop.
+//
+// Work is split over the cache's length.  The tiles of all (sequence, key head)
+// items form one line, and worker w of W takes the tiles [w n / W, (w + 1) n / W)
+// of it, whatever items they belong to: ragged batches and single long sequences
+// fill the card alike, without the host knowing a length.  A worker's first and
+// last item may be shared with its neighbours; their parts (maximum, sum and
+// unnormalised output) go to its two workspace slots and a second launch joins
+// them in order.  Sequences of length 0 count one empty tile and get zeros.
 // ---------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
 template <typename T>
-__global__ __launch_bounds__(256) void paged_attend_simple_k(const PagedAttendArgs a) {
-  constexpr int MAXD = 8;  // dim <= 512
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long b = blockIdx.x / a.heads;
-  const int h = (int)(blockIdx.x % a.heads);
-  const int kv = h / (a.heads / a.kv_heads);
+struct Matrix;
+
+template <>
+struct Matrix<__bf16> {
+  typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mul(V8 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <>
+struct Matrix<_Float16> {
+  typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mul(V8 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// A value that is the same in every lane of the wave, as the compiler's scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+  const int lo = uniform((int)x), hi = uniform((int)(x >> 32));
+  return ((long)hi << 32) | (unsigned)lo;
+}
+
+struct AttendPlan {
+  int workers;     // 0: one workgroup per item, nothing shared
+  int blocks;      // head blocks of 16 per key head
+  float* part;     // [2 * workers][min(16, G)][dim] unnormalised outputs
+  float* part_ms;  // [2 * workers][min(16, G)][2] maximum and sum
+};
+
+__device__ __forceinline__ int tiles_of(const PagedAttendArgs& a, long b, int tile) {
   long len = whole(a.lengths, a.lengths_i64, b);
   const long room = (long)a.cache.table_cols << a.cache.page_shift;
   len = len < room ? len : room;
-  const T* q = (const T*)a.q + b * a.q_batch + h * a.q_head;
-  float qv[MAXD], acc[MAXD] = {};
-#pragma unroll
-  for (int i = 0; i < MAXD; ++i) qv[i] = lane + 64 * i < a.dim ? (float)q[lane + 64 * i] : 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (long key = wave; key < len; key += 4) {
-    const long page = a.cache.table[b * a.cache.table_stride + (key >> a.cache.page_shift)];
-    if (page < 0 || page >= a.cache.pages) continue;
-    const long slot = key & ((1 << a.cache.page_shift) - 1);
-    const T* k = (const T*)a.cache.k + page * a.cache.k_page + kv * a.cache.k_head + slot * a.cache.k_slot;
-    const T* v = (const T*)a.cache.v + page * a.cache.v_page + kv * a.cache.v_head + slot * a.cache.v_slot;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < MAXD; ++i)
-      if (lane + 64 * i < a.dim) s += qv[i] * (float)k[lane + 64 * i];
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    s *= a.scale;
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
-    const float p = s == -INFINITY ? 0.f : exp2f(s - top);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < MAXD; ++i)
-      if (lane + 64 * i < a.dim) acc[i] = acc[i] * keep + p * (float)v[lane + 64 * i];
+  return len > 0 ? (int)((len + tile - 1) / tile) : 1;
+}
+
+// Where tile `at` of the line (or, with `seq` >= 0, where sequence `seq`) lies.
+struct Spot {
+  long b;      // sequence
+  long first;  // place of its first tile in the line
+  int tiles;   // of one of its items
+};
+
+// One wave over the batch, 64 sequences at a time.
+__device__ __forceinline__ Spot spot_of(const PagedAttendArgs& a, long items_per_seq, int tile,
+                                        long at, long seq) {
+  const int lane = threadIdx.x & 63;
+  long before = 0;
+  for (long b0 = 0; b0 < a.batch; b0 += 64) {
+    const bool in = b0 + lane < a.batch;
+    const int mine = in ? tiles_of(a, b0 + lane, tile) : 0;
+    long upto = (long)mine * items_per_seq;
+    for (int off = 1; off < 64; off <<= 1) {
+      const long o = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += o;
+    }
+    const bool here = in && (seq >= 0 ? b0 + lane == seq : before + upto > at);
+    const unsigned long long hit = __ballot(here);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      const int tiles = __shfl(mine, l, 64);
+      return {uniform(b0 + l), uniform(before + __shfl(upto, l, 64) - (long)tiles * items_per_seq),
+              uniform(tiles)};
+    }
+    before = uniform(before + __shfl(upto, 63, 64));
   }
-  __shared__ float sm[4], sl[4], sacc[4][512];
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
+  return {a.batch, before, 0};
+}
+
+__device__ __forceinline__ long tiles_in_all(const PagedAttendArgs& a, long items_per_seq, int tile) {
+  long n = 0;
+  for (long b = threadIdx.x & 63; b < a.batch; b += 64) n += tiles_of(a, b, tile);
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  return uniform(n) * items_per_seq;
+}
+
+// Workers that get work: at least one tile to each of a workgroup's waves.
+__device__ __forceinline__ long busy_workers(long workers, long total, int waves) {
+  const long most = (total + waves - 1) / waves;
+  return workers < most ? workers : most;
+}
+
+// The dim that the next smaller DP takes: chunks below it are never past `dim`.
+template <int DP>
+constexpr int smaller_dim() {
+  return DP <= 64 ? 0 : DP <= 96 ? 64 : DP <= 128 ? 96 : DP <= 192 ? 128 : 192;
+}
+
+// What one wave carries through its tiles of one item.
+template <typename T, int DP>
+struct Tiles;
+
+// 16-bit caches: tiles of 32 keys.
+template <typename T, int DP>
+struct Tiles {
+  using V8 = typename Matrix<T>::V8;
+  static constexpr int KEYS = 32;
+  static constexpr int J = DP / 32;
+  // a row of V in shared memory, padded so that the transposing read of 16 rows
+  // and the 16-byte writes of 16 rows both spread over all banks
+  static constexpr int PITCH = DP + 16;
+  static constexpr int LDS_BYTES = KEYS * PITCH * 2;
+  // whether chunks of column block j can lie past `dim`
+  static constexpr bool edge(int j) { return 32 * j + 32 > smaller_dim<DP>(); }
+  V8 q[J], k[2][J], v[2][J];
+  f32x4 acc[DP / 16];
+  float m, l;
+
+  __device__ __forceinline__ void start(const T* qrow, bool live, int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int i = 0; i < MAXD; ++i)
-    if (lane + 64 * i < a.dim) sacc[wave][lane + 64 * i] = acc[i];
-  __syncthreads();
-  float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float f[4], total = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - top);
-    total += f[w] * sl[w];
+    for (int j = 0; j < J; ++j) {
+      const int d = (chunk + 4 * j) * 8;
+      q[j] = V8{};
+      if (live && d < dim) q[j] = *(const V8*)(qrow + d);
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  T* out = (T*)a.out + (b * a.heads + h) * a.dim;
-  for (int d = threadIdx.x; d < a.dim; d += 256) {
-    float o = 0.f;
-    for (int w = 0; w < 4; ++w) o += f[w] * sacc[w][d];
-    out[d] = (T)(o * inv);
+
+  template <bool EXACT>
+  __device__ __forceinline__ void fetch(V8 (&x)[2][J], const T* base, const long (&row)[2], int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const T* p = base + row[h];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int d = (chunk + 4 * j) * 8;
+        // columns past dim: the row's first ones again, cleared before use
+        x[h][j] = *(const V8*)(p + (EXACT || !edge(j) || d < dim ? d : 0));
+      }
+    }
+  }
+
+  template <bool EXACT>
+  __device__ __forceinline__ void scores(f32x4 (&s)[2], int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        V8 x = k[h][j];
+        if (!EXACT && edge(j) && (chunk + 4 * j) * 8 >= dim) x = V8{};
+        s[h] = Matrix<T>::mul(x, q[j], s[h]);
+      }
+    }
+  }
+
+  // `ok`: bit i of ok[h] says that key 16 h + i counts.
+  __device__ __forceinline__ void weigh(f32x4 (&s)[2], float scale, const unsigned (&ok)[2], bool full,
+                                        V8& hi, V8& lo) {
+    const int group = (threadIdx.x & 63) >> 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[h][r] *= scale;
+        if (!full && !((ok[h] >> (4 * group + r)) & 1)) s[h][r] = -INFINITY;
+        top = fmaxf(top, s[h][r]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m)) {
+      const float next = fmaxf(m, top);
+      const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) acc[i] *= keep;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(s[h][r] - off);
+        l += p;
+        hi[4 * h + r] = (T)p;
+        lo[4 * h + r] = (T)(p - (float)hi[4 * h + r]);
+      }
+  }
+
+  __device__ __forceinline__ void stage(T* lds, const unsigned (&ok)[2], bool full) {
+    const int lane = threadIdx.x & 63, row = lane & 15, chunk = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool clear = !full && !((ok[h] >> row) & 1);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        *(V8*)(lds + (16 * h + row) * PITCH + (chunk + 4 * j) * 8) = clear ? V8{} : v[h][j];
+    }
+  }
+
+  __device__ __forceinline__ void gather(const T* lds, V8 hi, V8 lo) {
+    const int lane = threadIdx.x & 63, i = lane & 15, group = lane >> 4;
+    const T* p = lds + (4 * group + i / 4) * PITCH + (i % 4) * 4;
+    typedef __attribute__((address_space(3))) s16x4* Shared;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      union {
+        s16x4 half[2];
+        V8 all;
+      } x;
+      x.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(p + 16 * d));
+      x.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(p + 16 * PITCH + 16 * d));
+      acc[d] = Matrix<T>::mul(x.all, hi, acc[d]);
+      acc[d] = Matrix<T>::mul(x.all, lo, acc[d]);
+    }
+  }
+};
+
+// Orders a wave's own shared-memory writes before its reads of other lanes'
+// values, and the other way round.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int DP, bool EXACT>
+__device__ __forceinline__ void run_tiles(Tiles<T, DP>& w, const PagedAttendArgs& a, long b, int kv,
+                                          int len, int t, int end, int step, T* lds) {
+  constexpr int KEYS = Tiles<T, DP>::KEYS;
+  const int row = threadIdx.x & 15;
+  const int* table = a.cache.table + b * a.cache.table_stride;
+  const T* kbase = (const T*)a.cache.k + kv * a.cache.k_head;
+  const T* vbase = (const T*)a.cache.v + kv * a.cache.v_head;
+  const int slot_mask = (1 << a.cache.page_shift) - 1;
+  int page[2];
+  unsigned ok[2], ok_next[2];
+  long krow[2], vrow[2];
+  auto pages = [&](int tile) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = tile * KEYS + 16 * h + row;
+      page[h] = key < len ? table[key >> a.cache.page_shift] : -1;
+    }
+  };
+  // rows to read of a tile; keys that do not count read the cache's first row
+  auto resolve = [&](int tile, unsigned (&good)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = tile * KEYS + 16 * h + row;
+      const bool fine = page[h] >= 0 && page[h] < a.cache.pages;
+      const long slot = key & slot_mask;
+      krow[h] = fine ? page[h] * a.cache.k_page + slot * a.cache.k_slot : 0;
+      vrow[h] = fine ? page[h] * a.cache.v_page + slot * a.cache.v_slot : 0;
+      good[h] = (unsigned)__ballot(fine) & 0xffffu;
+    }
+  };
+  if (t >= end) return;
+  pages(t);
+  resolve(t, ok);
+  if (t + step < end) pages(t + step);
+  w.template fetch<EXACT>(w.k, kbase, krow, a.dim);
+  w.template fetch<EXACT>(w.v, vbase, vrow, a.dim);
+  for (; t < end; t += step) {
+    const bool more = t + step < end;
+    if (more) {
+      resolve(t + step, ok_next);
+      if (t + 2 * step < end) pages(t + 2 * step);  // ahead of the loads that follow
+    }
+    f32x4 s[2];
+    typename Tiles<T, DP>::V8 hi, lo;
+    w.template scores<EXACT>(s, a.dim);
+    if (more) w.template fetch<EXACT>(w.k, kbase, krow, a.dim);
+    const bool full = (ok[0] & ok[1]) == 0xffffu;
+    w.weigh(s, a.scale, ok, full, hi, lo);
+    w.stage(lds, ok, full);
+    if (more) w.template fetch<EXACT>(w.v, vbase, vrow, a.dim);
+    wave_sync();
+    w.gather(lds, hi, lo);
+    wave_sync();
+    ok[0] = ok_next[0];
+    ok[1] = ok_next[1];
   }
 }
 
+// float32 caches: tiles of 16 keys, the fp32 matrix instruction.
+template <int DP>
+struct Tiles<float, DP> {
+  static constexpr int KEYS = 16;
+  static constexpr int J = DP / 16;
+  static constexpr int LDS_BYTES = 16 * (DP + 4) * 4;  // the join's only
+  static constexpr bool edge(int j) { return 16 * j + 16 > smaller_dim<DP>(); }
+  f32x4 q[J], k[J], v[J], acc[J];  // v[d][r]: dim 16 d + l % 16 of key 4 (l / 16) + r
+  float m, l;
+
+  __device__ __forceinline__ void start(const float* qrow, bool live, int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int d = (chunk + 4 * j) * 4;
+      q[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (live && d < dim) q[j] = *(const f32x4*)(qrow + d);
+      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    m = -INFINITY;
+    l = 0.f;
+  }
+};
+
+template <int DP, bool EXACT>
+__device__ __forceinline__ void run_tiles_f32(Tiles<float, DP>& w, const PagedAttendArgs& a, long b,
+                                              int kv, int len, int t, int end, int step) {
+  constexpr int J = DP / 16;
+  const int lane = threadIdx.x & 63, row = lane & 15, chunk = lane >> 4;
+  const int* table = a.cache.table + b * a.cache.table_stride;
+  const float* kbase = (const float*)a.cache.k + kv * a.cache.k_head;
+  const float* vbase = (const float*)a.cache.v + kv * a.cache.v_head;
+  const int slot_mask = (1 << a.cache.page_shift) - 1;
+  int page = -1;
+  unsigned ok = 0, ok_next = 0;
+  long krow = 0, vrow = 0;
+  auto pages = [&](int tile) {
+    const int key = tile * 16 + row;
+    page = key < len ? table[key >> a.cache.page_shift] : -1;
+  };
+  auto resolve = [&](int tile, unsigned& good) {
+    const int key = tile * 16 + row;
+    const bool fine = page >= 0 && page < a.cache.pages;
+    const long slot = key & slot_mask;
+    krow = fine ? page * a.cache.k_page + slot * a.cache.k_slot : 0;
+    vrow = fine ? page * a.cache.v_page + slot * a.cache.v_slot : 0;
+    good = (unsigned)__ballot(fine) & 0xffffu;
+  };
+  auto fetch_k = [&]() {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int d = (chunk + 4 * j) * 4;
+      w.k[j] = *(const f32x4*)(kbase + krow + (EXACT || !w.edge(j) || d < a.dim ? d : 0));
+    }
+  };
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float* p = vbase + __shfl(vrow, 4 * chunk + r, 64);
+#pragma unroll
+      for (int d = 0; d < J; ++d) {
+        const int col = 16 * d + row;
+        w.v[d][r] = p[EXACT || !w.edge(d) || col < a.dim ? col : 0];
+      }
+    }
+  };
+  if (t >= end) return;
+  pages(t);
+  resolve(t, ok);
+  if (t + step < end) pages(t + step);
+  fetch_k();
+  fetch_v();
+  for (; t < end; t += step) {
+    const bool more = t + step < end;
+    if (more) {
+      resolve(t + step, ok_next);
+      if (t + 2 * step < end) pages(t + 2 * step);
+    }
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      f32x4 x = w.k[j];
+      if (!EXACT && w.edge(j) && (chunk + 4 * j) * 4 >= a.dim) x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w.q[j][i], s, 0, 0, 0);
+    }
+    if (more) fetch_k();
+    const bool full = ok == 0xffffu;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] *= a.scale;
+      if (!full && !((ok >> (4 * chunk + r)) & 1)) s[r] = -INFINITY;
+      top = fmaxf(top, s[r]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > w.m)) {
+      const float next = fmaxf(w.m, top);
+      const float keep = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - next);
+      w.m = next;
+      w.l *= keep;
+#pragma unroll
+      for (int i = 0; i < J; ++i) w.acc[i] *= keep;
+    }
+    const float off = w.m == -INFINITY ? 0.f : w.m;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float p = __builtin_amdgcn_exp2f(s[r] - off);
+      w.l += p;
+      const bool gone = !full && !((ok >> (4 * chunk + r)) & 1);
+#pragma unroll
+      for (int d = 0; d < J; ++d)
+        w.acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(gone ? 0.f : w.v[d][r], p, w.acc[d], 0, 0, 0);
+    }
+    if (more) fetch_v();
+    ok = ok_next;
+  }
+}
+
+template <typename T, int DP, bool EXACT, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : sizeof(T) == 2 ? 2 : 1) void paged_attend_k(
+    const PagedAttendArgs a, const AttendPlan plan) {
+  using W = Tiles<T, DP>;
+  constexpr int OUT = DP + 4;  // pitch of a head's output in shared memory
+  static_assert(16 * OUT * 4 <= W::LDS_BYTES, "the join reuses the staging rows");
+  __shared__ __attribute__((aligned(16))) char lds[NW][W::LDS_BYTES];
+  __shared__ float sm[NW][16], sl[NW][16];
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int group = a.heads / a.kv_heads;
+  const int per = a.kv_heads * plan.blocks;  // items of a sequence
+  const int rows = group < 16 ? group : 16;
+  const long room = (long)a.cache.table_cols << a.cache.page_shift;
+
+  long b;
+  int item, tiles, at, left;  // `left`: tiles still to do, over items
+  if (plan.workers == 0) {
+    b = blockIdx.x / per;
+    item = (int)(blockIdx.x % per);
+    tiles = left = tiles_of(a, b, W::KEYS);
+    at = 0;
+  } else {
+    const long total = tiles_in_all(a, per, W::KEYS);
+    const long busy = busy_workers(plan.workers, total, NW);
+    if (blockIdx.x >= busy) return;
+    const long lo = blockIdx.x * total / busy, hi = (blockIdx.x + 1) * total / busy;
+    const Spot s = spot_of(a, per, W::KEYS, lo, -1);
+    b = s.b;
+    tiles = s.tiles;
+    item = (int)((lo - s.first) / tiles);
+    at = (int)((lo - s.first) % tiles);
+    left = (int)(hi - lo);
+  }
+  bool first = true;
+  while (left > 0) {
+    const int end = left < tiles - at ? at + left : tiles;
+    long len = whole(a.lengths, a.lengths_i64, b);
+    len = len < room ? len : room;
+    const int kv = item / plan.blocks;
+    const int head0 = kv * group + 16 * (item % plan.blocks);  // the first of this block
+    const int heads = min(16, (kv + 1) * group - head0);
+    W w;
+    const bool live = (lane & 15) < heads;
+    w.start((const T*)a.q + b * a.q_batch + (head0 + (live ? lane & 15 : 0)) * a.q_head, live, a.dim);
+    if constexpr (sizeof(T) == 4)
+      run_tiles_f32<DP, EXACT>(w, a, b, kv, (int)len, at + wave, end, NW);
+    else
+      run_tiles<T, DP, EXACT>(w, a, b, kv, (int)len, at + wave, end, NW, (T*)lds[wave]);
+    w.l += __shfl_xor(w.l, 16, 64);
+    w.l += __shfl_xor(w.l, 32, 64);
+    wave_sync();
+    float* mine = (float*)lds[wave] + (lane & 15) * OUT + 4 * (lane >> 4);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) *(f32x4*)(mine + 16 * d) = w.acc[d];
+    if (lane < 16) {
+      sm[wave][lane] = w.m;
+      sl[wave][lane] = w.l;
+    }
+    __syncthreads();
+    const bool shared = at > 0 || end < tiles;
+    const long slot = 2 * (long)blockIdx.x + (first ? 0 : 1);
+    for (int i = threadIdx.x; i < heads * a.dim; i += 64 * NW) {
+      const int g = i / a.dim, d = i - g * a.dim;
+      float top = sm[0][g];
+#pragma unroll
+      for (int o = 1; o < NW; ++o) top = fmaxf(top, sm[o][g]);
+      float sum = 0.f, out = 0.f;
+#pragma unroll
+      for (int o = 0; o < NW; ++o) {
+        const float f = sm[o][g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[o][g] - top);
+        sum += f * sl[o][g];
+        out += f * ((const float*)lds[o])[g * OUT + d];
+      }
+      if (shared) {
+        plan.part[(slot * rows + g) * a.dim + d] = out;
+        if (d == 0) {
+          plan.part_ms[(slot * rows + g) * 2] = top;
+          plan.part_ms[(slot * rows + g) * 2 + 1] = sum;
+        }
+      } else {
+        ((T*)a.out)[(b * a.heads + head0 + g) * a.dim + d] = (T)(sum == 0.f ? 0.f : out / sum);
+      }
+    }
+    first = false;
+    left -= end - at;
+    at = 0;
+    if (left > 0) {
+      __syncthreads();  // the rows above are staged into again
+      if (++item == per) {
+        item = 0;
+        ++b;
+        tiles = tiles_of(a, b, W::KEYS);
+      }
+    }
+  }
+}
+
+// Joins the parts of items that several workers shared: blockIdx.x is the item,
+// or where there are more items than workers the border between two workers;
+// blockIdx.y a head's 64 dims.  Four groups of lanes take every fourth part.
 template <typename T>
-int attend_simple(const PagedAttendArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attend_simple_k<T>), dim3((unsigned)(a.batch * a.heads)), dim3(256), 0,
-                     st, a);
+__global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs a, const AttendPlan plan,
+                                                           int tile, int waves, int by_item) {
+  const int group = a.heads / a.kv_heads;
+  const int per = a.kv_heads * plan.blocks;
+  const int rows = group < 16 ? group : 16;
+  const int chunks = (a.dim + 63) / 64;
+  const int g = blockIdx.y / chunks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int d = (blockIdx.y % chunks) * 64 + lane;
+  const long total = tiles_in_all(a, per, tile);
+  const long busy = busy_workers(plan.workers, total, waves);
+  Spot s;
+  int item;
+  if (by_item) {
+    s = spot_of(a, per, tile, 0, blockIdx.x / per);
+    item = (int)(blockIdx.x % per);
+  } else {
+    const long border = blockIdx.x + 1;
+    if (border >= busy) return;
+    const long lo = border * total / busy;
+    s = spot_of(a, per, tile, lo, -1);
+    item = (int)((lo - s.first) / s.tiles);
+    const long from = s.first + (long)item * s.tiles;
+    // only the first border strictly inside an item joins it
+    if (lo == from || (border - 1) * total / busy > from) return;
+  }
+  const long from = s.first + (long)item * s.tiles, to = from + s.tiles;
+  const long w0 = ((from + 1) * busy - 1) / total, w1 = (to * busy - 1) / total;
+  if (w0 == w1) return;  // one worker had it all and wrote it
+  const int kv = item / plan.blocks;
+  const int head = kv * group + 16 * (item % plan.blocks) + g;
+  if (head >= (kv + 1) * group) return;
+  __shared__ float sm[4], sl[4], so[4][64];
+  float top = -INFINITY, sum = 0.f, out = 0.f;
+  for (long w = w0 + wave; w <= w1; w += 4) {
+    // the worker's first slot if its range begins in this item
+    const long slot = 2 * w + (w * total / busy >= from ? 0 : 1);
+    const float m = plan.part_ms[(slot * rows + g) * 2], l = plan.part_ms[(slot * rows + g) * 2 + 1];
+    const float x = d < a.dim ? plan.part[(slot * rows + g) * a.dim + d] : 0.f;
+    if (m == -INFINITY && !(l != l)) continue;  // no key of this part counted
+    const float next = fmaxf(top, m);
+    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    const float f = __builtin_amdgcn_exp2f(m - next);
+    top = next;
+    sum = sum * keep + f * l;
+    out = out * keep + f * x;
+  }
+  if (lane == 0) {
+    sm[wave] = top;
+    sl[wave] = sum;
+  }
+  so[wave][lane] = out;
+  __syncthreads();
+  if (wave != 0 || d >= a.dim) return;
+  const float all = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  sum = out = 0.f;
+#pragma unroll
+  for (int o = 0; o < 4; ++o) {
+    const float f = sm[o] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[o] - all);
+    sum += f * sl[o];
+    out += f * so[o][lane];
+  }
+  ((T*)a.out)[(s.b * a.heads + head) * a.dim + d] = (T)(sum == 0.f ? 0.f : out / sum);
+}
+
+template <typename T, int DP, bool EXACT>
+int attend_launch(const PagedAttendArgs& a, hipStream_t st) {
+  constexpr int KEYS = Tiles<T, DP>::KEYS;
+  const AttendPlan plan{a.workers, a.head_blocks, a.part, a.part_ms};
+  const int per = a.kv_heads * a.head_blocks;
+  const long items = a.batch * per;
+  if (a.workers == 0) {
+    if (a.waves == 1)
+      hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 1>), dim3((unsigned)items), dim3(64), 0, st, a, plan);
+    else
+      hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), dim3((unsigned)items), dim3(256), 0, st, a, plan);
+    return (int)hipGetLastError();
+  }
+  hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), dim3((unsigned)a.workers), dim3(256), 0, st, a, plan);
+  const int group = a.heads / a.kv_heads;
+  const int by_item = items < a.workers;
+  const dim3 grid((unsigned)(by_item ? items : a.workers - 1),
+                  (unsigned)((group < 16 ? group : 16) * ((a.dim + 63) / 64)));
+  if (grid.x)
+    hipLaunchKernelGGL((paged_attend_join_k<T>), grid, dim3(256), 0, st, a, plan, KEYS, 4, by_item);
   return (int)hipGetLastError();
 }
 
+template <typename T, int DP>
+int attend_dim(const PagedAttendArgs& a, hipStream_t st) {
+  return a.dim == DP ? attend_launch<T, DP, true>(a, st) : attend_launch<T, DP, false>(a, st);
+}
+
+template <typename T>
+int attend_any(const PagedAttendArgs& a, hipStream_t st) {
+  if (a.dim <= 64) return attend_dim<T, 64>(a, st);
+  if (a.dim <= 96) return attend_dim<T, 96>(a, st);
+  if (a.dim <= 128) return attend_dim<T, 128>(a, st);
+  if (a.dim <= 192) return attend_dim<T, 192>(a, st);
+  return attend_dim<T, 256>(a, st);
+}
+
 }  // namespace
+
+// How a call is split, by what the host knows: the table's columns bound every
+// length.
+extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
+  const int keys = a->dtype == RL_F32 ? 16 : 32;
+  const long room = (long)a->cache.table_cols << a->cache.page_shift;
+  const long most = (room + keys - 1) / keys;  // tiles of an item
+  const int group = a->heads / a->kv_heads;
+  a->head_blocks = (group + 15) / 16;
+  const long items = a->batch * a->kv_heads * a->head_blocks;
+  if (most <= 8) {
+    a->workers = 0;
+    a->waves = items >= 1024 ? 1 : 4;
+    return;
+  }
+  const long resident = (long)cus * (a->dim <= 128 ? 3 : a->dtype == RL_F32 ? 1 : 2);
+  const long worth = (items * most + 3) / 4;
+  a->workers = (int)(resident < worth ? resident : worth);
+  a->waves = 4;
+}
 
 extern "C" int launch_paged_append(const PagedAppendArgs* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
@@ -291,11 +885,11 @@ extern "C" int launch_paged_attend(const PagedAttendArgs* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   switch (a->dtype) {
     case RL_F32:
-      return attend_simple<float>(*a, st);
+      return attend_any<float>(*a, st);
     case RL_BF16:
-      return attend_simple<__bf16>(*a, st);
+      return attend_any<__bf16>(*a, st);
     case RL_F16:
-      return attend_simple<_Float16>(*a, st);
+      return attend_any<_Float16>(*a, st);
   }
   return (int)hipErrorInvalidValue;
 }
