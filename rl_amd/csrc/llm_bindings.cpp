@@ -614,8 +614,10 @@ Tensor paged_attention_decode(const Tensor& q_in, const Tensor& k_cache, const T
   Tensor part;
   if (a.workers) {
     const int64_t rows = 2 * (int64_t)a.workers * std::min(16, a.heads / a.kv_heads);
-    part = torch::empty({rows * (a.dim + 2)}, q.options().dtype(torch::kFloat32));
-    a.part = part.data_ptr<float>();
+    const int64_t notes = a.workers * paged_attend_note_bytes() / 4;
+    part = torch::empty({notes + rows * (a.dim + 2)}, q.options().dtype(torch::kFloat32));
+    a.notes = part.data_ptr<float>();
+    a.part = part.data_ptr<float>() + notes;
     a.part_ms = a.part + rows * a.dim;
   }
   launched(launch_paged_attend(&a, stream_of()), "paged_attention_decode");

@@ -53,10 +53,12 @@ struct PagedAttendArgs {
   // workspace where workers > 0
   float* part;             // [2 * workers][min(16, heads / kv_heads)][dim]
   float* part_ms;          // [2 * workers][min(16, heads / kv_heads)][2]
+  void* notes;             // [workers] of paged_attend_note_bytes()
 };
 
 extern "C" {
 int launch_paged_append(const PagedAppendArgs* a, void* stream);
+long paged_attend_note_bytes(void);
 void plan_paged_attend(PagedAttendArgs* a, int cus);
 int launch_paged_attend(const PagedAttendArgs* a, void* stream);
 }

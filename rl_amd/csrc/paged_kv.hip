@@ -262,9 +262,16 @@ __device__ __forceinline__ long uniform(long x) {
   return ((long)hi << 32) | (unsigned)lo;
 }
 
+// An item that several workers shared; parts == 0: none begins here.
+struct SharedItem {
+  long b;
+  int item, worker, parts, slot;  // the first part's worker and slot
+};
+
 struct AttendPlan {
   int workers;     // 0: one workgroup per item, nothing shared
   int blocks;      // head blocks of 16 per key head
+  SharedItem* notes;  // [workers]
   float* part;     // [2 * workers][min(16, G)][dim] unnormalised outputs
   float* part_ms;  // [2 * workers][min(16, G)][2] maximum and sum
 };
@@ -276,44 +283,71 @@ __device__ __forceinline__ int tiles_of(const PagedAttendArgs& a, long b, int ti
   return len > 0 ? (int)((len + tile - 1) / tile) : 1;
 }
 
-// Where tile `at` of the line (or, with `seq` >= 0, where sequence `seq`) lies.
+// Where sequence `b` and its items lie on the line of all tiles.
 struct Spot {
-  long b;      // sequence
-  long first;  // place of its first tile in the line
+  long b;
+  long first;  // place of its first tile
   int tiles;   // of one of its items
 };
 
-// One wave over the batch, 64 sequences at a time.
-__device__ __forceinline__ Spot spot_of(const PagedAttendArgs& a, long items_per_seq, int tile,
-                                        long at, long seq) {
+// The line as one wave sees it: up to 64 sequences in its lanes, more in passes.
+struct Line {
+  int mine;   // tiles of an item of sequence `lane` (batches up to 64)
+  long upto;  // inclusive sum over sequences, times the items of a sequence
+  long total;
+};
+
+__device__ __forceinline__ void line_pass(const PagedAttendArgs& a, long per, int tile, long b0,
+                                          Line& x) {
+  const int lane = threadIdx.x & 63;
+  x.mine = b0 + lane < a.batch ? tiles_of(a, b0 + lane, tile) : 0;
+  x.upto = (long)x.mine * per;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const long o = __shfl_up(x.upto, off, 64);
+    if (lane >= off) x.upto += o;
+  }
+}
+
+__device__ __forceinline__ Line line_of(const PagedAttendArgs& a, long per, int tile) {
+  Line x;
+  if (a.batch <= 64) {
+    line_pass(a, per, tile, 0, x);
+    x.total = uniform(__shfl(x.upto, 63, 64));
+    return x;
+  }
+  long n = 0;
+  for (long b = threadIdx.x & 63; b < a.batch; b += 64) n += tiles_of(a, b, tile);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  x.mine = 0;
+  x.upto = 0;
+  x.total = uniform(n) * per;
+  return x;
+}
+
+// The sequence of tile `at`.
+__device__ __forceinline__ Spot spot_of(const PagedAttendArgs& a, long per, int tile, Line x, long at) {
   const int lane = threadIdx.x & 63;
   long before = 0;
   for (long b0 = 0; b0 < a.batch; b0 += 64) {
-    const bool in = b0 + lane < a.batch;
-    const int mine = in ? tiles_of(a, b0 + lane, tile) : 0;
-    long upto = (long)mine * items_per_seq;
-    for (int off = 1; off < 64; off <<= 1) {
-      const long o = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += o;
-    }
-    const bool here = in && (seq >= 0 ? b0 + lane == seq : before + upto > at);
+    if (a.batch > 64) line_pass(a, per, tile, b0, x);
+    const bool here = b0 + lane < a.batch && before + x.upto > at;
     const unsigned long long hit = __ballot(here);
     if (hit) {
       const int l = __ffsll((long long)hit) - 1;
-      const int tiles = __shfl(mine, l, 64);
-      return {uniform(b0 + l), uniform(before + __shfl(upto, l, 64) - (long)tiles * items_per_seq),
-              uniform(tiles)};
+      const int tiles = uniform(__shfl(x.mine, l, 64));
+      return {uniform(b0 + l), before + uniform(__shfl(x.upto, l, 64)) - (long)tiles * per, tiles};
     }
-    before = uniform(before + __shfl(upto, 63, 64));
+    before += uniform(__shfl(x.upto, 63, 64));
   }
-  return {a.batch, before, 0};
+  return {a.batch, before, 1};  // not reached: `at` < total
 }
 
-__device__ __forceinline__ long tiles_in_all(const PagedAttendArgs& a, long items_per_seq, int tile) {
-  long n = 0;
-  for (long b = threadIdx.x & 63; b < a.batch; b += 64) n += tiles_of(a, b, tile);
-  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-  return uniform(n) * items_per_seq;
+// x * y / z of whole numbers, 64-bit divisions only where 32 bits do not hold.
+__device__ __forceinline__ long share(long x, long y, long z) {
+  const long p = x * y;
+  return (p | z) < (1L << 32) ? (long)((unsigned)p / (unsigned)z) : p / z;
 }
 
 // Workers that get work: at least one tile to each of a workgroup's waves.
@@ -643,8 +677,13 @@ __device__ __forceinline__ void run_tiles_f32(Tiles<float, DP>& w, const PagedAt
   }
 }
 
+// Waves to a SIMD that the registers are held to.
+constexpr int resident_waves(int dim, int size) {
+  return dim <= 96 ? 3 : dim <= 128 || (size == 2 && dim <= 192) ? 2 : 1;
+}
+
 template <typename T, int DP, bool EXACT, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : sizeof(T) == 2 ? 2 : 1) void paged_attend_k(
+__global__ __launch_bounds__(64 * NW, resident_waves(DP, sizeof(T))) void paged_attend_k(
     const PagedAttendArgs a, const AttendPlan plan) {
   using W = Tiles<T, DP>;
   constexpr int OUT = DP + 4;  // pitch of a head's output in shared memory
@@ -659,22 +698,39 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : sizeof(T) == 2 ? 2 : 1) vo
 
   long b;
   int item, tiles, at, left;  // `left`: tiles still to do, over items
+  SharedItem note = {0, 0, 0, 0, 0};
   if (plan.workers == 0) {
     b = blockIdx.x / per;
     item = (int)(blockIdx.x % per);
     tiles = left = tiles_of(a, b, W::KEYS);
     at = 0;
   } else {
-    const long total = tiles_in_all(a, per, W::KEYS);
-    const long busy = busy_workers(plan.workers, total, NW);
-    if (blockIdx.x >= busy) return;
-    const long lo = blockIdx.x * total / busy, hi = (blockIdx.x + 1) * total / busy;
-    const Spot s = spot_of(a, per, W::KEYS, lo, -1);
+    const Line line = line_of(a, per, W::KEYS);
+    const long busy = busy_workers(plan.workers, line.total, NW);
+    if (blockIdx.x >= busy) {
+      if (threadIdx.x == 0) plan.notes[blockIdx.x] = note;
+      return;
+    }
+    const long lo = share(blockIdx.x, line.total, busy), hi = share(blockIdx.x + 1, line.total, busy);
+    const Spot s = spot_of(a, per, W::KEYS, line, lo);
     b = s.b;
     tiles = s.tiles;
-    item = (int)((lo - s.first) / tiles);
-    at = (int)((lo - s.first) % tiles);
+    item = (int)share(lo - s.first, 1, tiles);
+    at = (int)(lo - s.first - (long)item * tiles);
     left = (int)(hi - lo);
+    if (at > 0) {
+      // the first border strictly inside an item answers for its join
+      const long from = lo - at, before = share(blockIdx.x - 1, line.total, busy);
+      if (before <= from) {
+        // the worker of the item's last tile is the last whose range begins at or
+        // before it: ceil(end * busy / total) - 1
+        const long end = from + tiles, last = share(end, busy, line.total);
+        const int w1 = (int)(last * line.total == end * busy ? last - 1 : last);
+        note = {b, item, (int)blockIdx.x - 1, w1 - (int)blockIdx.x + 2,
+                2 * ((int)blockIdx.x - 1) + (before == from ? 0 : 1)};
+      }
+    }
+    if (threadIdx.x == 0) plan.notes[blockIdx.x] = note;
   }
   bool first = true;
   while (left > 0) {
@@ -740,95 +796,92 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : sizeof(T) == 2 ? 2 : 1) vo
   }
 }
 
-// Joins the parts of items that several workers shared: blockIdx.x is the item,
-// or where there are more items than workers the border between two workers;
-// blockIdx.y a head's 64 dims.  Four groups of lanes take every fourth part.
+// Joins the parts of an item that several workers shared, by the note that the
+// first worker whose range begins inside the item left (blockIdx.x).  blockIdx.y
+// takes 128 of the item's values (heads x dims), 4 to a lane; the 8 half-waves
+// take every eighth part each, eight at a time, so that an item of 64 parts waits
+// for its loads once.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs a, const AttendPlan plan,
-                                                           int tile, int waves, int by_item) {
+__global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs a, const AttendPlan plan) {
+  __shared__ float sm[8][32], sl[8][32];
+  __shared__ f32x4 so[8][32];
+  const SharedItem note = plan.notes[blockIdx.x];
+  if (note.parts == 0) return;
   const int group = a.heads / a.kv_heads;
-  const int per = a.kv_heads * plan.blocks;
   const int rows = group < 16 ? group : 16;
-  const int chunks = (a.dim + 63) / 64;
-  const int g = blockIdx.y / chunks;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int d = (blockIdx.y % chunks) * 64 + lane;
-  const long total = tiles_in_all(a, per, tile);
-  const long busy = busy_workers(plan.workers, total, waves);
-  Spot s;
-  int item;
-  if (by_item) {
-    s = spot_of(a, per, tile, 0, blockIdx.x / per);
-    item = (int)(blockIdx.x % per);
-  } else {
-    const long border = blockIdx.x + 1;
-    if (border >= busy) return;
-    const long lo = border * total / busy;
-    s = spot_of(a, per, tile, lo, -1);
-    item = (int)((lo - s.first) / s.tiles);
-    const long from = s.first + (long)item * s.tiles;
-    // only the first border strictly inside an item joins it
-    if (lo == from || (border - 1) * total / busy > from) return;
-  }
-  const long from = s.first + (long)item * s.tiles, to = from + s.tiles;
-  const long w0 = ((from + 1) * busy - 1) / total, w1 = (to * busy - 1) / total;
-  if (w0 == w1) return;  // one worker had it all and wrote it
-  const int kv = item / plan.blocks;
-  const int head = kv * group + 16 * (item % plan.blocks) + g;
-  if (head >= (kv + 1) * group) return;
-  __shared__ float sm[4], sl[4], so[4][64];
-  float top = -INFINITY, sum = 0.f, out = 0.f;
-  for (long w = w0 + wave; w <= w1; w += 4) {
-    // the worker's first slot if its range begins in this item
-    const long slot = 2 * w + (w * total / busy >= from ? 0 : 1);
-    const float m = plan.part_ms[(slot * rows + g) * 2], l = plan.part_ms[(slot * rows + g) * 2 + 1];
-    const float x = d < a.dim ? plan.part[(slot * rows + g) * a.dim + d] : 0.f;
-    if (m == -INFINITY && !(l != l)) continue;  // no key of this part counted
-    const float next = fmaxf(top, m);
-    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
-    const float f = __builtin_amdgcn_exp2f(m - next);
-    top = next;
-    sum = sum * keep + f * l;
-    out = out * keep + f * x;
-  }
-  if (lane == 0) {
-    sm[wave] = top;
-    sl[wave] = sum;
-  }
-  so[wave][lane] = out;
-  __syncthreads();
-  if (wave != 0 || d >= a.dim) return;
-  const float all = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  sum = out = 0.f;
+  const int kv = note.item / plan.blocks;
+  const int head0 = kv * group + 16 * (note.item % plan.blocks);
+  const int heads = min(16, (kv + 1) * group - head0);
+  const int quads = a.dim / 4;
+  const int half = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int q = blockIdx.y * 32 + lane;
+  const int g = min(q / quads, heads - 1);  // lanes past the item repeat its last head
+  const int quad = q % quads;
+  float top = -INFINITY, sum = 0.f;
+  f32x4 out = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 8;
+  for (int i0 = half; i0 < note.parts; i0 += 8 * N) {
+    float m[N], l[N];
+    f32x4 x[N];
 #pragma unroll
-  for (int o = 0; o < 4; ++o) {
-    const float f = sm[o] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[o] - all);
-    sum += f * sl[o];
+    for (int u = 0; u < N; ++u) {
+      const int i = min(i0 + 8 * u, note.parts - 1);
+      // all but the first part lie in their workers' first slots
+      const long row = (i == 0 ? note.slot : 2 * (long)(note.worker + i)) * rows + g;
+      m[u] = plan.part_ms[2 * row];
+      l[u] = plan.part_ms[2 * row + 1];
+      x[u] = *(const f32x4*)(plan.part + row * a.dim + 4 * quad);
+    }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < N; ++u) next = fmaxf(next, m[u]);
+    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    top = next;
+    sum *= keep;
+    out *= keep;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (i0 + 8 * u >= note.parts) continue;
+      const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+      sum += f * l[u];
+      out += f * x[u];
+    }
+  }
+  sm[half][lane] = top;
+  sl[half][lane] = sum;
+  so[half][lane] = out;
+  __syncthreads();
+  if (half != 0 || q >= heads * quads) return;
+#pragma unroll
+  for (int o = 1; o < 8; ++o) top = fmaxf(top, sm[o][lane]);
+  sum = 0.f;
+  out = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int o = 0; o < 8; ++o) {
+    const float m = sm[o][lane];
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    sum += f * sl[o][lane];
     out += f * so[o][lane];
   }
-  ((T*)a.out)[(s.b * a.heads + head) * a.dim + d] = (T)(sum == 0.f ? 0.f : out / sum);
+  T* dst = (T*)a.out + (note.b * a.heads + head0 + g) * a.dim + 4 * quad;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) dst[r] = (T)(sum == 0.f ? 0.f : out[r] / sum);
 }
 
 template <typename T, int DP, bool EXACT>
 int attend_launch(const PagedAttendArgs& a, hipStream_t st) {
-  constexpr int KEYS = Tiles<T, DP>::KEYS;
-  const AttendPlan plan{a.workers, a.head_blocks, a.part, a.part_ms};
+  const AttendPlan plan{a.workers, a.head_blocks, (SharedItem*)a.notes, a.part, a.part_ms};
   const int per = a.kv_heads * a.head_blocks;
   const long items = a.batch * per;
-  if (a.workers == 0) {
-    if (a.waves == 1)
-      hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 1>), dim3((unsigned)items), dim3(64), 0, st, a, plan);
-    else
-      hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), dim3((unsigned)items), dim3(256), 0, st, a, plan);
-    return (int)hipGetLastError();
-  }
-  hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), dim3((unsigned)a.workers), dim3(256), 0, st, a, plan);
+  const dim3 blocks((unsigned)(a.workers ? a.workers : items));
+  if (a.waves == 1)
+    hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 1>), blocks, dim3(64), 0, st, a, plan);
+  else
+    hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), blocks, dim3(256), 0, st, a, plan);
+  if (a.workers < 2) return (int)hipGetLastError();
   const int group = a.heads / a.kv_heads;
-  const int by_item = items < a.workers;
-  const dim3 grid((unsigned)(by_item ? items : a.workers - 1),
-                  (unsigned)((group < 16 ? group : 16) * ((a.dim + 63) / 64)));
-  if (grid.x)
-    hipLaunchKernelGGL((paged_attend_join_k<T>), grid, dim3(256), 0, st, a, plan, KEYS, 4, by_item);
+  const dim3 grid((unsigned)a.workers, (unsigned)(((group < 16 ? group : 16) * a.dim + 127) / 128));
+  hipLaunchKernelGGL((paged_attend_join_k<T>), grid, dim3(256), 0, st, a, plan);
   return (int)hipGetLastError();
 }
 
@@ -848,8 +901,21 @@ int attend_any(const PagedAttendArgs& a, hipStream_t st) {
 
 }  // namespace
 
+extern "C" long paged_attend_note_bytes(void) { return (long)sizeof(SharedItem); }
+
 // How a call is split, by what the host knows: the table's columns bound every
-// length.
+// length.  Measured in us, 16-bit caches, the other choice in brackets:
+//
+// - Short tables take one workgroup per item and no join, of one wave where
+//   there are items to fill the card: 2048 items of 16 tiles 99 [split: 108],
+//   3072 of 16 74 [80]; 4096 of 4 tiles 57 [four waves: 74].  Longer ones are
+//   split, for ragged batches: what a direct call wins at equal lengths (768
+//   items of 32 tiles 39 [43]) it loses on the longest item of others.
+// - A split call gives a CU one workgroup of 4 waves for dims above 96, where
+//   their tiles on the way (128 dim bytes to a wave) cover the latency, and two
+//   below: 1 x 131072 keys, 8 heads of 128: 101 [104 with two, 113 with three];
+//   2 heads of 256, 65536 keys: 40 [54]; 48 x 4096, 12 heads of 64: 113 [120
+//   with one].  More workers only add prologues and parts to join.
 extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   const int keys = a->dtype == RL_F32 ? 16 : 32;
   const long room = (long)a->cache.table_cols << a->cache.page_shift;
@@ -857,13 +923,13 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   const int group = a->heads / a->kv_heads;
   a->head_blocks = (group + 15) / 16;
   const long items = a->batch * a->kv_heads * a->head_blocks;
-  if (most <= 8) {
+  if (most <= 8 || (most <= 16 && items >= 1024)) {
     a->workers = 0;
     a->waves = items >= 1024 ? 1 : 4;
     return;
   }
-  const long resident = (long)cus * (a->dim <= 128 ? 3 : a->dtype == RL_F32 ? 1 : 2);
-  const long worth = (items * most + 3) / 4;
+  const long resident = (long)cus * (a->dim > 96 ? 1 : 2);
+  const long worth = (items * most + 3) / 4;  // a tile to each wave
   a->workers = (int)(resident < worth ? resident : worth);
   a->waves = 4;
 }

@@ -42,6 +42,8 @@ struct PolicyOperand {
 struct PolicyLossArgs {
   PolicyOperand log_probs, old_log_probs, advantage, mask, ref;
   long rows, cols;
+  unsigned cols_magic;     // the launcher's: reciprocal of cols
+  int cols_shift;
   int variant;             // 0: clipped surrogate, 1: clipped weight
   double log_low, log_high;    // borders of the log ratio
   double log_off;              // upper border of the clip_fraction count
@@ -50,7 +52,7 @@ struct PolicyLossArgs {
   int mean;                // 1: divide by the mask's sum, 0: plain sums
   double* partials;        // [blocks][8]
   int blocks;
-  float* out;              // 7 floats at out[i * out_stride]
+  float* out;              // 7 scalars
   float* scale;            // 1 / denominator, for the backward pass
   // backward
   const float* g_total;    // upstream scalars; null: zero

@@ -165,10 +165,16 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_fwd_k(const TokenLogPro
         for (int u = 0; u < U; ++u) load16<T>(body + (long)(v + u * TPR) * N, x[u]);
         absorb<U, N>(r, x, c);
       }
-      for (; v < vecs; v += TPR) {
-        float x[1][N];
-        load16<T>(body + (long)v * N, x[0]);
-        absorb<1, N>(r, x, c);
+      if (v < vecs) {  // what is left, all loads at once: the row's last vector for none
+        float x[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, vecs - 1) * N, x[u]);
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+          if (v + u * TPR >= vecs)
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[u][i] = -INFINITY;
+        absorb<U, N>(r, x, c);
       }
     }
 #pragma unroll
@@ -258,10 +264,13 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
 #pragma unroll
       for (int u = 0; u < U; ++u) finish(v + u * TPR, x[u]);
     }
-    for (; v < vecs; v += TPR) {
-      float x[N];
-      load16<T>(body + (long)v * N, x);
-      finish(v, x);
+    if (v < vecs) {  // what is left, all loads at once
+      float x[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, vecs - 1) * N, x[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + u * TPR < vecs) finish(v + u * TPR, x[u]);
     }
   }
 }
@@ -280,12 +289,24 @@ int log_probs_launch(const TokenLogProbArgs& a, bool bwd, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// Threads to a row, by the row's bytes (MI355X, bf16, 8192 rows, forward /
+// backward, us):
+//             64 threads   256      512      1024
+//    2.4 KB    14 / 13   18 / 19  35 / 41   55 / 63
+//     10 KB    24 / 30   25 / 29  48 / 48   74 / 74
+//     32 KB    47 / 98   46 / 89  57 / 98   91 / 117
+//     64 KB    97 / 193  99 / 188 90 / 173 111 / 170
+//    100 KB   146 / 311 146 / 301 137 / 287 158 / 270
+// and for 256 rows of 10 KB, too few for a wave each, 7.4 / 7.4 with 64 threads
+// and 6.2 / 6.3 with 256.
 template <typename T>
 int log_probs_dispatch(const TokenLogProbArgs& a, bool bwd, hipStream_t st) {
   const long bytes = (long)a.vocab * (long)sizeof(T);
-  if (bytes <= 4096) return log_probs_launch<T, 64, 256, 4>(a, bwd, st);
-  if (a.rows >= 1024) return log_probs_launch<T, 256, 256, 4>(a, bwd, st);
-  return log_probs_launch<T, 1024, 1024, 4>(a, bwd, st);
+  if (bytes <= 4096 || (bytes <= 8192 && a.rows >= 1024))
+    return log_probs_launch<T, 64, 256, 8>(a, bwd, st);
+  if (bytes <= 40960) return log_probs_launch<T, 256, 256, 4>(a, bwd, st);
+  return bwd ? log_probs_launch<T, 1024, 1024, 4>(a, bwd, st)
+             : log_probs_launch<T, 512, 512, 4>(a, bwd, st);
 }
 
 int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
@@ -312,17 +333,21 @@ int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
 //   entropy term: + lp (the sampled estimate of -H); d/dlp = 1
 //   objective = -sum w gain / D, and the rest likewise
 //
-// Whether a ratio is clipped is decided in double on x against the borders'
-// logarithms: x is then exact for fp32 inputs, and an element next to a border
-// falls on the same side as in the definition.  e^y - 1 - y cancels near 0: a
-// series there.  Sums are in double (the loop is bound by its loads).
+// Whether a ratio is clipped is decided on x against the borders' logarithms,
+// in double where float32 could fall on the other side, so that an element next
+// to a border is treated as in the definition.  e^y - 1 - y cancels near 0: a
+// series there.  Four tokens are summed in float32, what follows in double.
 //
-// One workgroup does everything up to 16K tokens; above, partial sums of many
-// and a second launch that joins them in a fixed order: no atomics, the result
-// does not depend on the order of execution.  Launch bound below ~1M tokens.
+// One workgroup does everything up to 16K tokens (two launches cost more than
+// its few passes); above, partial sums of many and a second launch that joins
+// them in a fixed order: no atomics, the result does not depend on the order of
+// execution.  Dense operands take 4 tokens to an access; any other strides or
+// types go one by one through the runtime codes.  The row of a token (for an
+// advantage per row) comes from a multiplication by the column count's
+// reciprocal; 64-bit divisions took longer than the loads.
 // ---------------------------------------------------------------------------
 
-__device__ __forceinline__ double operand(const PolicyOperand& o, long r, long c) {
+__device__ __forceinline__ float operand(const PolicyOperand& o, long r, long c) {
   const long i = r * o.stride_row + c * o.stride_col;
   switch (o.dtype) {
     case RL_F32:
@@ -334,24 +359,23 @@ __device__ __forceinline__ double operand(const PolicyOperand& o, long r, long c
     case RL_U8:
       return ((const unsigned char*)o.ptr)[i];
     case RL_I32:
-      return ((const int*)o.ptr)[i];
+      return (float)((const int*)o.ptr)[i];
     case RL_I64:
-      return (double)((const long*)o.ptr)[i];
+      return (float)((const long*)o.ptr)[i];
     case RL_I8:
       return ((const signed char*)o.ptr)[i];
     case RL_I16:
       return ((const short*)o.ptr)[i];
     default:
-      return ((const double*)o.ptr)[i];
+      return (float)((const double*)o.ptr)[i];
   }
 }
 
 // e^y - 1 - y
 __device__ __forceinline__ float kl3(float y) {
-  if (fabsf(y) > 0.5f) return expf(y) - 1.f - y;
+  if (fabsf(y) > 0.5f) return exp2_hw(y * kLog2e) - 1.f - y;
   // y^2 (1/2! + y/3! + y^2/4! + ...), remainder below 2^-25 of the sum at 1/2
-  float p = 1.f / 3628800.f;
-  p = fmaf(p, y, 1.f / 362880.f);
+  float p = 1.f / 362880.f;
   p = fmaf(p, y, 1.f / 40320.f);
   p = fmaf(p, y, 1.f / 5040.f);
   p = fmaf(p, y, 1.f / 720.f);
@@ -363,16 +387,27 @@ __device__ __forceinline__ float kl3(float y) {
 }
 
 struct PolicyToken {
-  bool above, below;
+  bool above, below, off;
   float x, ratio;
 };
 
-__device__ __forceinline__ PolicyToken policy_token(const PolicyLossArgs& a, double x) {
+__device__ __forceinline__ PolicyToken policy_token(const PolicyLossArgs& a, float lp, float old) {
   PolicyToken t;
-  t.above = x > a.log_high;
-  t.below = x < a.log_low;
-  t.x = (float)x;
-  t.ratio = expf(t.x);
+  t.x = lp - old;
+  const float lo = (float)a.log_low, hi = (float)a.log_high, off = (float)a.log_off;
+  t.above = t.x > hi;
+  t.below = t.x < lo;
+  t.off = t.x > off;
+  // the difference and the borders are each rounded once: 2^-21 is 4 times that
+  const float near = 4.76837158e-7f * fmaxf(1.f, fabsf(t.x));
+  if (fabsf(t.x - hi) < near || fabsf(t.x - lo) < near || fabsf(t.x - off) < near) {
+    const double x = (double)lp - (double)old;
+    t.above = x > a.log_high;
+    t.below = x < a.log_low;
+    t.off = x > a.log_off;
+  }
+  t.off = t.off || t.below;
+  t.ratio = exp2_hw(t.x * kLog2e);
   return t;
 }
 
@@ -381,6 +416,40 @@ __device__ __forceinline__ bool clipped_against(const PolicyToken& t, float adv)
 }
 
 enum { S_GAIN, S_KL, S_LP, S_W, S_R, S_RR, S_OFF, S_COUNT };
+
+// One token's terms, added to float sums of a few tokens.
+__device__ __forceinline__ void policy_terms(const PolicyLossArgs& a, float lp, float old, float adv,
+                                             float w, float ref, bool has_ref, float (&s)[S_COUNT]) {
+  const PolicyToken t = policy_token(a, lp, old);
+  s[S_R] += t.ratio;
+  s[S_RR] += t.ratio * t.ratio;
+  s[S_OFF] += t.off ? 1.f : 0.f;
+  if (w == 0.f) return;  // a masked token may hold anything, NaN too
+  const float bound = t.above ? a.high : t.below ? a.low : t.ratio;
+  const float gain = a.variant == 0 ? (clipped_against(t, adv) ? bound : t.ratio) * adv
+                                    : bound * t.x * adv;
+  s[S_GAIN] += w * gain;
+  s[S_W] += w;
+  s[S_LP] += w * lp;
+  if (has_ref) s[S_KL] += w * kl3(ref - lp);
+}
+
+// What a token's gradient is, before its upstream factors are folded in:
+// go, gk and ge carry the upstream gradients, coefficients and 1 / D.
+__device__ __forceinline__ float policy_grad(const PolicyLossArgs& a, float lp, float old, float adv,
+                                             float w, float ref, bool has_ref, float go, float gk,
+                                             float ge) {
+  if (w == 0.f) return 0.f;
+  const PolicyToken t = policy_token(a, lp, old);
+  const float dgain = a.variant == 0 ? (clipped_against(t, adv) ? 0.f : t.ratio * adv)
+                                     : (t.above ? a.high : t.below ? a.low : t.ratio) * adv;
+  float d = ge - go * dgain;
+  if (has_ref) {
+    const float y = ref - lp;
+    d -= gk * (kl3(y) + y);
+  }
+  return d * w;
+}
 
 __device__ __forceinline__ void policy_finish(const PolicyLossArgs& a, const double (&s)[S_COUNT]) {
   const double n = (double)a.rows * (double)a.cols;
@@ -402,44 +471,99 @@ template <int BLOCK>
 __device__ __forceinline__ bool block_sums(double (&s)[S_COUNT]) {
   __shared__ double part[BLOCK / 64][S_COUNT];
 #pragma unroll
-  for (int k = 0; k < S_COUNT; ++k)
-    for (int off = 32; off > 0; off >>= 1) s[k] += __shfl_xor(s[k], off, 64);
+  for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < S_COUNT; ++k) s[k] += __shfl_xor(s[k], off, 64);
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
     for (int k = 0; k < S_COUNT; ++k) part[threadIdx.x >> 6][k] = s[k];
   __syncthreads();
   if (threadIdx.x != 0) return false;
+#pragma unroll
   for (int w = 1; w < BLOCK / 64; ++w)
 #pragma unroll
     for (int k = 0; k < S_COUNT; ++k) s[k] += part[w][k];
   return true;
 }
 
-template <int BLOCK>
-__global__ __launch_bounds__(BLOCK) void policy_loss_fwd_k(const PolicyLossArgs a) {
+// n / cols for n < 2^31.
+__device__ __forceinline__ unsigned row_of(const PolicyLossArgs& a, unsigned n) {
+  return (__umulhi(a.cols_magic, n) + n) >> a.cols_shift;
+}
+
+// Four tokens of dense operands.
+struct Four {
+  float lp[4], old[4], ref[4], adv[4], w[4];
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const void* p, unsigned i, float (&x)[4]) {
+  struct alignas(4 * sizeof(T)) Q {
+    T x[4];
+  };
+  const Q q = *(const Q*)((const T*)p + i);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = (float)q.x[k];
+}
+
+template <typename T>
+__device__ __forceinline__ void load_four(const PolicyLossArgs& a, unsigned i, unsigned n, Four& f) {
+  if (i + 4 <= n) {
+    load4<T>(a.log_probs.ptr, i, f.lp);
+    load4<T>(a.old_log_probs.ptr, i, f.old);
+    if (a.ref.ptr) load4<T>(a.ref.ptr, i, f.ref);
+    if (a.mask.ptr) load4<unsigned char>(a.mask.ptr, i, f.w);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned j = i + k < n ? i + k : n - 1;
+      f.lp[k] = (float)((const T*)a.log_probs.ptr)[j];
+      f.old[k] = (float)((const T*)a.old_log_probs.ptr)[j];
+      if (a.ref.ptr) f.ref[k] = (float)((const T*)a.ref.ptr)[j];
+      if (a.mask.ptr) f.w[k] = ((const unsigned char*)a.mask.ptr)[j];
+    }
+  }
+  if (!a.mask.ptr) f.w[0] = f.w[1] = f.w[2] = f.w[3] = 1.f;
+  if (a.advantage.stride_col) {  // one for each token
+    const float* adv = (const float*)a.advantage.ptr;
+    if (i + 4 <= n) {
+      load4<float>(adv, i, f.adv);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f.adv[k] = adv[i + k < n ? i + k : n - 1];
+    }
+    return;
+  }
+  // one for each row: a single value unless the four cross into the next
+  unsigned r = row_of(a, i), c = i - r * (unsigned)a.cols;
+  const float* adv = (const float*)a.advantage.ptr;
+  f.adv[0] = adv[(long)r * a.advantage.stride_row];
+  if (c + 4 <= (unsigned)a.cols) {
+    f.adv[1] = f.adv[2] = f.adv[3] = f.adv[0];
+  } else {
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      if (++c == (unsigned)a.cols) c = 0, ++r;
+      f.adv[k] = adv[(long)(r < (unsigned)a.rows ? r : 0) * a.advantage.stride_row];
+    }
+  }
+}
+
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void policy_loss_dense_fwd_k(const PolicyLossArgs a) {
   double s[S_COUNT] = {};
-  const long n = a.rows * a.cols;
-  for (long i = (long)blockIdx.x * BLOCK + threadIdx.x; i < n; i += (long)gridDim.x * BLOCK) {
-    const long r = i / a.cols, c = i - r * a.cols;
-    const double lp = operand(a.log_probs, r, c);
-    const double x = lp - operand(a.old_log_probs, r, c);
-    const PolicyToken t = policy_token(a, x);
-    s[S_R] += t.ratio;
-    s[S_RR] += (double)t.ratio * t.ratio;
-    s[S_OFF] += (x > a.log_off || t.below) ? 1.0 : 0.0;
-    const double w = a.mask.ptr ? operand(a.mask, r, c) : 1.0;
-    if (w == 0.0) continue;  // a masked token may hold anything, NaN too
-    const float adv = (float)operand(a.advantage, r, c);
-    const float bound = t.above ? a.high : t.below ? a.low : t.ratio;
-    float gain;
-    if (a.variant == 0)
-      gain = (clipped_against(t, adv) ? bound : t.ratio) * adv;
-    else
-      gain = bound * t.x * adv;
-    s[S_GAIN] += w * gain;
-    s[S_W] += w;
-    s[S_LP] += w * lp;
-    if (a.ref.ptr) s[S_KL] += w * kl3((float)(operand(a.ref, r, c) - lp));
+  const unsigned n = (unsigned)(a.rows * a.cols);
+  const bool has_ref = a.ref.ptr != nullptr;
+  for (unsigned i = 4 * (blockIdx.x * BLOCK + threadIdx.x); i < n; i += 4 * gridDim.x * BLOCK) {
+    Four f;
+    load_four<T>(a, i, n, f);
+    float part[S_COUNT] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n)
+        policy_terms(a, f.lp[k], f.old[k], f.adv[k], f.w[k], has_ref ? f.ref[k] : 0.f, has_ref, part);
+#pragma unroll
+    for (int k = 0; k < S_COUNT; ++k) s[k] += part[k];
   }
   if (!block_sums<BLOCK>(s)) return;
   if (gridDim.x == 1) {
@@ -450,41 +574,137 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_fwd_k(const PolicyLossArgs 
   for (int k = 0; k < S_COUNT; ++k) a.partials[(long)blockIdx.x * 8 + k] = s[k];
 }
 
-__global__ __launch_bounds__(256) void policy_loss_join_k(const PolicyLossArgs a) {
+template <int BLOCK>
+__global__ __launch_bounds__(BLOCK) void policy_loss_fwd_k(const PolicyLossArgs a) {
   double s[S_COUNT] = {};
-  for (int b = threadIdx.x; b < a.blocks; b += 256)
+  const long n = a.rows * a.cols;
+  const bool has_ref = a.ref.ptr != nullptr;
+  for (long i = (long)blockIdx.x * BLOCK + threadIdx.x; i < n; i += (long)gridDim.x * BLOCK) {
+    const long r = n < (1L << 31) ? row_of(a, (unsigned)i) : i / a.cols, c = i - r * a.cols;
+    float part[S_COUNT] = {};
+    policy_terms(a, operand(a.log_probs, r, c), operand(a.old_log_probs, r, c),
+                 operand(a.advantage, r, c), a.mask.ptr ? operand(a.mask, r, c) : 1.f,
+                 has_ref ? operand(a.ref, r, c) : 0.f, has_ref, part);
+#pragma unroll
+    for (int k = 0; k < S_COUNT; ++k) s[k] += part[k];
+  }
+  if (!block_sums<BLOCK>(s)) return;
+  if (gridDim.x == 1) {
+    policy_finish(a, s);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < S_COUNT; ++k) a.partials[(long)blockIdx.x * 8 + k] = s[k];
+}
+
+__global__ __launch_bounds__(512) void policy_loss_join_k(const PolicyLossArgs a) {
+  double s[S_COUNT] = {};
+  for (int b = threadIdx.x; b < a.blocks; b += 512)
 #pragma unroll
     for (int k = 0; k < S_COUNT; ++k) s[k] += a.partials[(long)b * 8 + k];
-  if (block_sums<256>(s)) policy_finish(a, s);
+  if (block_sums<512>(s)) policy_finish(a, s);
+}
+
+struct PolicyUpstream {
+  float go, gk, ge;
+};
+
+__device__ __forceinline__ PolicyUpstream policy_upstream(const PolicyLossArgs& a) {
+  const float inv = *a.scale;
+  const float total = a.g_total ? *a.g_total : 0.f;
+  return {(total + (a.g_objective ? *a.g_objective : 0.f)) * inv,
+          (total + (a.g_kl ? *a.g_kl : 0.f)) * a.kl_coeff * inv,
+          (total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void policy_loss_dense_bwd_k(const PolicyLossArgs a) {
+  const PolicyUpstream u = policy_upstream(a);
+  const unsigned n = (unsigned)(a.rows * a.cols);
+  const bool has_ref = a.ref.ptr != nullptr && a.kl_coeff != 0.f;
+  struct alignas(4 * sizeof(T)) Q {
+    T x[4];
+  };
+  for (unsigned i = 4 * (blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * gridDim.x * 256) {
+    Four f;
+    load_four<T>(a, i, n, f);
+    Q q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      q.x[k] = (T)policy_grad(a, f.lp[k], f.old[k], f.adv[k], f.w[k], has_ref ? f.ref[k] : 0.f, has_ref,
+                              u.go, u.gk, u.ge);
+    if (i + 4 <= n) {
+      *(Q*)((T*)a.grad + i) = q;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) ((T*)a.grad)[i + k] = q.x[k];
+    }
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void policy_loss_bwd_k(const PolicyLossArgs a) {
-  const float inv = *a.scale;
-  const float total = a.g_total ? *a.g_total : 0.f;
-  const float go = (total + (a.g_objective ? *a.g_objective : 0.f)) * inv;
-  const float gk = (total + (a.g_kl ? *a.g_kl : 0.f)) * a.kl_coeff * inv;
-  const float ge = (total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv;
+  const PolicyUpstream u = policy_upstream(a);
   const long n = a.rows * a.cols;
+  const bool has_ref = a.ref.ptr != nullptr && a.kl_coeff != 0.f;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-    const long r = i / a.cols, c = i - r * a.cols;
-    const float w = a.mask.ptr ? (float)operand(a.mask, r, c) : 1.f;
-    float d = 0.f;
-    if (w != 0.f) {
-      const double lp = operand(a.log_probs, r, c);
-      const PolicyToken t = policy_token(a, lp - operand(a.old_log_probs, r, c));
-      const float adv = (float)operand(a.advantage, r, c);
-      float dgain;
-      if (a.variant == 0)
-        dgain = clipped_against(t, adv) ? 0.f : t.ratio * adv;
-      else
-        dgain = (t.above ? a.high : t.below ? a.low : t.ratio) * adv;
-      d = ge - go * dgain;
-      if (a.ref.ptr && a.kl_coeff != 0.f) d -= gk * expm1f((float)(operand(a.ref, r, c) - lp));
-      d *= w;
-    }
-    ((T*)a.grad)[i] = (T)d;
+    const long r = n < (1L << 31) ? row_of(a, (unsigned)i) : i / a.cols, c = i - r * a.cols;
+    ((T*)a.grad)[i] = (T)policy_grad(a, operand(a.log_probs, r, c), operand(a.old_log_probs, r, c),
+                                     operand(a.advantage, r, c), a.mask.ptr ? operand(a.mask, r, c) : 1.f,
+                                     has_ref ? operand(a.ref, r, c) : 0.f, has_ref, u.go, u.gk, u.ge);
   }
+}
+
+// Whether the dense kernels may take the operands: 4 tokens to an access.
+bool policy_dense(const PolicyLossArgs& a) {
+  const long n = a.rows * a.cols;
+  auto dense = [&](const PolicyOperand& o, int dtype, long align) {
+    return o.dtype == dtype && (o.stride_col == 1 || a.cols == 1) &&
+           (o.stride_row == a.cols || a.rows == 1) && (size_t)o.ptr % align == 0;
+  };
+  const int t = a.log_probs.dtype;
+  const long align = t == RL_F32 ? 16 : 8;
+  return n < (1L << 31) - (1L << 22) && dense(a.log_probs, t, align) && dense(a.old_log_probs, t, align) &&
+         (!a.ref.ptr || dense(a.ref, t, align)) && (!a.mask.ptr || dense(a.mask, RL_U8, 4)) &&
+         (dense(a.advantage, RL_F32, 16) ||
+          (a.advantage.dtype == RL_F32 && a.advantage.stride_col == 0));
+}
+
+// The reciprocal for row_of: with s = ceil(log2 d), magic = 2^32 (2^s - d) / d + 1.
+void policy_divisor(PolicyLossArgs* a) {
+  const unsigned long d = (unsigned long)a->cols;
+  if (d >= (1ul << 31)) return;  // no 32-bit index is used then
+  int s = 0;
+  while ((1ul << s) < d) ++s;
+  a->cols_shift = s;
+  a->cols_magic = (unsigned)(((1ul << 32) * ((1ul << s) - d)) / d + 1);
+}
+
+template <typename T>
+int policy_bwd(const PolicyLossArgs& a, hipStream_t st) {
+  const long n = a.rows * a.cols;
+  const bool dense = policy_dense(a);
+  const long need = dense ? (n + 1023) / 1024 : (n + 255) / 256;
+  const dim3 grid((unsigned)(need < 4096 ? need : 4096));
+  if (dense)
+    hipLaunchKernelGGL((policy_loss_dense_bwd_k<T>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((policy_loss_bwd_k<T>), grid, dim3(256), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+template <int BLOCK>
+void policy_fwd_block(const PolicyLossArgs& a, bool dense, hipStream_t st) {
+  const dim3 grid(a.blocks), block(BLOCK);
+  if (!dense)
+    hipLaunchKernelGGL((policy_loss_fwd_k<BLOCK>), grid, block, 0, st, a);
+  else if (a.log_probs.dtype == RL_F32)
+    hipLaunchKernelGGL((policy_loss_dense_fwd_k<float, BLOCK>), grid, block, 0, st, a);
+  else if (a.log_probs.dtype == RL_BF16)
+    hipLaunchKernelGGL((policy_loss_dense_fwd_k<__bf16, BLOCK>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((policy_loss_dense_fwd_k<_Float16, BLOCK>), grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -500,40 +720,36 @@ extern "C" int launch_token_log_probs_bwd(const TokenLogProbArgs* a, void* strea
 extern "C" int policy_loss_blocks(long n) {
   if (n <= 16384) return 1;
   const long b = (n + 2047) / 2048;
-  return (int)(b < 1024 ? b : 1024);
+  return (int)(b < 512 ? b : 512);
 }
 
-extern "C" int launch_policy_loss_fwd(const PolicyLossArgs* a, void* stream) {
+extern "C" int launch_policy_loss_fwd(const PolicyLossArgs* args, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  if (a->blocks == 1) {
-    if (a->rows * a->cols <= 256)
-      hipLaunchKernelGGL((policy_loss_fwd_k<256>), dim3(1), dim3(256), 0, st, *a);
-    else
-      hipLaunchKernelGGL((policy_loss_fwd_k<1024>), dim3(1), dim3(1024), 0, st, *a);
+  PolicyLossArgs a = *args;
+  policy_divisor(&a);
+  const bool dense = policy_dense(a);
+  if (a.blocks > 1) {
+    policy_fwd_block<512>(a, dense, st);
+    hipLaunchKernelGGL(policy_loss_join_k, dim3(1), dim3(512), 0, st, a);
+  } else if (a.rows * a.cols <= 1024) {
+    policy_fwd_block<256>(a, dense, st);
   } else {
-    hipLaunchKernelGGL((policy_loss_fwd_k<256>), dim3(a->blocks), dim3(256), 0, st, *a);
-    hipLaunchKernelGGL(policy_loss_join_k, dim3(1), dim3(256), 0, st, *a);
+    policy_fwd_block<1024>(a, dense, st);
   }
   return (int)hipGetLastError();
 }
 
-extern "C" int launch_policy_loss_bwd(const PolicyLossArgs* a, void* stream) {
+extern "C" int launch_policy_loss_bwd(const PolicyLossArgs* args, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const long n = a->rows * a->cols;
-  const long need = (n + 255) / 256;
-  const dim3 grid((unsigned)(need < 4096 ? need : 4096));
-  switch (a->log_probs.dtype) {
+  PolicyLossArgs a = *args;
+  policy_divisor(&a);
+  switch (a.log_probs.dtype) {
     case RL_F32:
-      hipLaunchKernelGGL((policy_loss_bwd_k<float>), grid, dim3(256), 0, st, *a);
-      break;
+      return policy_bwd<float>(a, st);
     case RL_BF16:
-      hipLaunchKernelGGL((policy_loss_bwd_k<__bf16>), grid, dim3(256), 0, st, *a);
-      break;
+      return policy_bwd<__bf16>(a, st);
     case RL_F16:
-      hipLaunchKernelGGL((policy_loss_bwd_k<_Float16>), grid, dim3(256), 0, st, *a);
-      break;
-    default:
-      return (int)hipErrorInvalidValue;
+      return policy_bwd<_Float16>(a, st);
   }
-  return (int)hipGetLastError();
+  return (int)hipErrorInvalidValue;
 }

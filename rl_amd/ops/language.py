@@ -20,6 +20,8 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
+from . import _C, _require_ext
+
 __all__ = [
     "TokenPolicyLoss",
     "paged_attention_decode",
@@ -35,8 +37,6 @@ _VARIANTS = {"clip": 0, "cispo": 1}
 def _ext(tensor: torch.Tensor):
     """The extension for a tensor: required on the GPU, its argument checks
     used on the CPU where it is built."""
-    from . import _C, _require_ext
-
     if tensor.is_cuda:
         _require_ext()
     return _C
