@@ -30,6 +30,7 @@ struct TokenLogProbArgs {
   float* stats;         // [rows][2]: the max and the sum of exp2; may be null in forward
   const float* upstream;  // [rows], backward
   void* grad;           // [rows][vocab] dense, backward
+  int stream_grad;      // the launcher's: write the gradient past the caches
 };
 
 // One operand of the policy loss seen as [rows][cols] with strides.

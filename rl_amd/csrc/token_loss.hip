@@ -73,11 +73,17 @@ __device__ __forceinline__ void load16<_Float16>(const _Float16* p, float (&x)[8
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&x)[Vec16<T>::N]) {
+__device__ __forceinline__ void store16(T* p, const float (&x)[Vec16<T>::N], bool stream) {
+  typedef unsigned U4 __attribute__((ext_vector_type(4)));
   T h[Vec16<T>::N];
 #pragma unroll
   for (int i = 0; i < Vec16<T>::N; ++i) h[i] = (T)x[i];
-  __builtin_memcpy(__builtin_assume_aligned(p, 16), h, 16);
+  U4 u;
+  __builtin_memcpy(&u, h, 16);
+  if (stream)
+    __builtin_nontemporal_store(u, (U4*)p);
+  else
+    *(U4*)p = u;
 }
 
 struct MaxSum {
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
       const float zero[N] = {};
       if (t < head) out[t] = (T)0.f;
       if (TPR - 1 - t < tail) out[a.vocab - (TPR - t)] = (T)0.f;
-      for (int v = t; v < vecs; v += TPR) store16<T>(obody + (long)v * N, zero);
+      for (int v = t; v < vecs; v += TPR) store16<T>(obody + (long)v * N, zero, a.stream_grad);
       continue;
     }
     const bool known = tok >= 0 && tok < a.vocab;
@@ -254,7 +260,7 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
         for (int i = 0; i < N; ++i)
           if (i == at) x[i] += g;
       }
-      store16<T>(obody + (long)v * N, x);
+      store16<T>(obody + (long)v * N, x, a.stream_grad);
     };
     int v = t;
     for (; v + (U - 1) * TPR < vecs; v += U * TPR) {
@@ -713,8 +719,14 @@ extern "C" int launch_token_log_probs_fwd(const TokenLogProbArgs* a, void* strea
   return log_probs_any(a, false, stream);
 }
 
-extern "C" int launch_token_log_probs_bwd(const TokenLogProbArgs* a, void* stream) {
-  return log_probs_any(a, true, stream);
+// A gradient that the last-level cache (256 MB) cannot hold next to its logits is
+// written past it: what it would push out is what the passes around it read, and
+// its own reader finds it in memory either way.  2048 x 50257 bf16 (206 MB),
+// forward + backward: 57 + 73 -> 42 + 69 us; 8192 rows: 172 + 276 -> 144 + 279.
+extern "C" int launch_token_log_probs_bwd(const TokenLogProbArgs* args, void* stream) {
+  TokenLogProbArgs a = *args;
+  a.stream_grad = a.rows * a.vocab * (a.dtype == RL_F32 ? 4 : 2) > (128L << 20);
+  return log_probs_any(&a, true, stream);
 }
 
 extern "C" int policy_loss_blocks(long n) {
