@@ -33,58 +33,52 @@ struct alignas(sizeof(T) * VEC) Chunk {
 };
 
 // One lane's place within a head: two chunks, rotated against each other
-// (interleaved: each within itself) or copied.
+// (interleaved: each within itself) or copied.  Either way the two belong to the
+// angles [item * VEC, (item + 1) * VEC).
 struct Place {
   int first, second;  // element offsets; second < 0: none
   bool turn;
-  int angle0, angle1;  // first column of the tables for each chunk
 };
 
 template <int VEC>
 __device__ __forceinline__ Place place_of(int item, int dim, int rotary, int interleaved) {
-  Place p;
   const int turning = rotary / 2 / VEC;
+  Place p;
   p.turn = item < turning;
-  if (p.turn && !interleaved) {
-    p.first = item * VEC;
-    p.second = p.first + rotary / 2;
-    p.angle0 = p.angle1 = item * VEC;
-  } else if (p.turn) {
-    p.first = 2 * item * VEC;
-    p.second = p.first + VEC;
-    p.angle0 = item * VEC;
-    p.angle1 = item * VEC + VEC / 2;
+  if (p.turn) {
+    p.first = interleaved ? 2 * item * VEC : item * VEC;
+    p.second = interleaved ? p.first + VEC : p.first + rotary / 2;
   } else {
     p.first = rotary + 2 * (item - turning) * VEC;
     p.second = p.first + VEC < dim ? p.first + VEC : -1;
-    p.angle0 = p.angle1 = 0;
   }
   return p;
 }
 
 template <int VEC>
-__device__ __forceinline__ int places(int dim, int rotary) {
+__host__ __device__ constexpr int places(int dim, int rotary) {
   return rotary / 2 / VEC + ((dim - rotary) / VEC + 1) / 2;
 }
 
-// LANES lanes share a head; 256 / LANES heads are worked on at once, of one
-// token, or of several when a token has fewer heads than that.
+// 1 << lanes_shift lanes share a head; the workgroup's slots take `per_token`
+// heads of a token at a time, and `tokens_here` tokens where those are all.  One
+// head on the way per thread and many threads: two or three heads at a time cost
+// registers and ran at 4.2 and 4.1 TB/s where this runs at 5.0 (32768 tokens of
+// 32 + 16 heads of 128, bf16).
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void paged_append_k(const PagedAppendArgs a, int lanes_shift,
-                                                      int tokens_shift) {
+                                                      int per_token, int tokens_here) {
   using C = Chunk<T, VEC>;
-  const int lanes = 1 << lanes_shift;
-  const int item = threadIdx.x & (lanes - 1);
-  const int slots = 256 >> lanes_shift;             // heads at once
-  const int per_token = slots >> tokens_shift;      // heads of one token at once
+  const int item = threadIdx.x & ((1 << lanes_shift) - 1);
   const int slot = threadIdx.x >> lanes_shift;
   const int rows = a.q ? a.heads : 0;
   const int all = rows + 2 * a.kv_heads;
   const int page_size = 1 << a.cache.page_shift;
   const long tokens = a.batch * a.width;
-  const long token = ((long)blockIdx.x << tokens_shift) + slot / per_token;
-  if (token >= tokens) return;
-  const long b = token / a.width;
+  const int sub = tokens_here > 1 ? slot / per_token : 0;
+  const long token = (long)blockIdx.x * tokens_here + sub;
+  if (token >= tokens || sub >= tokens_here) return;
+  const long b = (unsigned)token / (unsigned)a.width;  // at most 2^24 tokens
   const int t = (int)(token - b * a.width);
   const long length = a.lengths ? whole(a.lengths, a.lengths_i64, b) : a.width;
   const bool live = t < length;
@@ -102,73 +96,51 @@ __global__ __launch_bounds__(256) void paged_append_k(const PagedAppendArgs a, i
   const int plain = places<VEC>(a.dim, 0);
   const Place rot = place_of<VEC>(item, a.dim, a.rotary, a.interleaved);
   const Place copy = place_of<VEC>(item, a.dim, 0, 0);
-  float cs0[VEC], sn0[VEC], cs1[VEC], sn1[VEC];
-  if (a.rotary && rot.turn && item < turned && live) {
-    const bool inside = pos >= 0 && pos < a.positions;
-    const long row = inside ? pos * (a.rotary / 2) : 0;
+  float cs[VEC], sn[VEC];
+  if (a.rotary && rot.turn && live) {
+    if (pos >= 0 && pos < a.positions) {
+      __builtin_memcpy(cs, a.cos + pos * (a.rotary / 2) + item * VEC, sizeof(cs));
+      __builtin_memcpy(sn, a.sin + pos * (a.rotary / 2) + item * VEC, sizeof(sn));
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      // interleaved: element i of a chunk belongs to pair i / 2
-      const int j0 = a.interleaved ? rot.angle0 + i / 2 : rot.angle0 + i;
-      cs0[i] = inside ? a.cos[row + j0] : NAN;
-      sn0[i] = inside ? a.sin[row + j0] : NAN;
-      if (a.interleaved) {
-        const int j1 = rot.angle1 + i / 2;
-        cs1[i] = inside ? a.cos[row + j1] : NAN;
-        sn1[i] = inside ? a.sin[row + j1] : NAN;
-      }
+      for (int i = 0; i < VEC; ++i) cs[i] = sn[i] = NAN;
     }
   }
-  for (int h = slot % per_token; h < all; h += per_token) {
+  const T* qsrc = (const T*)a.q + b * a.q_batch + t * a.q_token;
+  const T* ksrc = (const T*)a.k + b * a.k_batch + t * a.k_token;
+  const T* vsrc = (const T*)a.v + b * a.v_batch + t * a.v_token;
+  T* qdst = (T*)a.q_out + token * a.heads * a.dim;
+  T* kdst = (T*)a.cache.k + page * a.cache.k_page + in_page * a.cache.k_slot;
+  T* vdst = (T*)a.cache.v + page * a.cache.v_page + in_page * a.cache.v_slot;
+  for (int h = slot - sub * per_token; h < all; h += per_token) {
     const bool is_q = h < rows, is_v = h >= rows + a.kv_heads;
+    if (item >= (is_v ? plain : turned) || (!is_q && page < 0)) continue;
     const Place p = is_v ? copy : rot;
-    if (item >= (is_v ? plain : turned)) continue;
-    const T* src;
-    T* dst;
-    if (is_q) {
-      src = (const T*)a.q + b * a.q_batch + t * a.q_token + h * a.q_head;
-      dst = (T*)a.q_out + (token * a.heads + h) * a.dim;
-    } else {
-      if (page < 0) continue;
-      if (is_v) {
-        const int g = h - rows - a.kv_heads;
-        src = (const T*)a.v + b * a.v_batch + t * a.v_token + g * a.v_head;
-        dst = (T*)a.cache.v + page * a.cache.v_page + g * a.cache.v_head +
-              in_page * a.cache.v_slot;
-      } else {
-        const int g = h - rows;
-        src = (const T*)a.k + b * a.k_batch + t * a.k_token + g * a.k_head;
-        dst = (T*)a.cache.k + page * a.cache.k_page + g * a.cache.k_head +
-              in_page * a.cache.k_slot;
-      }
-    }
+    const int g = is_q ? h : is_v ? h - rows - a.kv_heads : h - rows;
+    const T* src = is_q ? qsrc + g * a.q_head : is_v ? vsrc + g * a.v_head : ksrc + g * a.k_head;
+    T* dst = is_q ? qdst + g * a.dim : is_v ? vdst + g * a.cache.v_head : kdst + g * a.cache.k_head;
     C x{}, y{};
     if (live) {
       x = *(const C*)(src + p.first);
       if (p.second >= 0) y = *(const C*)(src + p.second);
-    }
-    if (live && !is_v && p.turn) {
-      if (a.interleaved) {
+      if (!is_v && p.turn) {
+        if (a.interleaved && VEC > 1) {
 #pragma unroll
-        for (int i = 0; i + 1 < VEC; i += 2) {
-          const float p0 = (float)x.x[i], p1 = (float)x.x[i + 1];
-          x.x[i] = (T)(p0 * cs0[i] - p1 * sn0[i]);
-          x.x[i + 1] = (T)(p1 * cs0[i] + p0 * sn0[i]);
-          const float r0 = (float)y.x[i], r1 = (float)y.x[i + 1];
-          y.x[i] = (T)(r0 * cs1[i] - r1 * sn1[i]);
-          y.x[i + 1] = (T)(r1 * cs1[i] + r0 * sn1[i]);
-        }
-        if (VEC == 1) {  // a pair is the two chunks
-          const float p0 = (float)x.x[0], p1 = (float)y.x[0];
-          x.x[0] = (T)(p0 * cs0[0] - p1 * sn0[0]);
-          y.x[0] = (T)(p1 * cs0[0] + p0 * sn0[0]);
-        }
-      } else {
+          for (int i = 0; i + 1 < VEC; i += 2) {
+            const float p0 = (float)x.x[i], p1 = (float)x.x[i + 1];
+            x.x[i] = (T)(p0 * cs[i / 2] - p1 * sn[i / 2]);
+            x.x[i + 1] = (T)(p1 * cs[i / 2] + p0 * sn[i / 2]);
+            const float r0 = (float)y.x[i], r1 = (float)y.x[i + 1];
+            y.x[i] = (T)(r0 * cs[VEC / 2 + i / 2] - r1 * sn[VEC / 2 + i / 2]);
+            y.x[i + 1] = (T)(r1 * cs[VEC / 2 + i / 2] + r0 * sn[VEC / 2 + i / 2]);
+          }
+        } else {  // the two chunks against each other (VEC 1: an interleaved pair too)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float p0 = (float)x.x[i], p1 = (float)y.x[i];
-          x.x[i] = (T)(p0 * cs0[i] - p1 * sn0[i]);
-          y.x[i] = (T)(p1 * cs0[i] + p0 * sn0[i]);
+          for (int i = 0; i < VEC; ++i) {
+            const float p0 = (float)x.x[i], p1 = (float)y.x[i];
+            x.x[i] = (T)(p0 * cs[i] - p1 * sn[i]);
+            y.x[i] = (T)(p1 * cs[i] + p0 * sn[i]);
+          }
         }
       }
     }
@@ -179,18 +151,31 @@ __global__ __launch_bounds__(256) void paged_append_k(const PagedAppendArgs a, i
 
 template <typename T, int VEC>
 int append_launch(const PagedAppendArgs& a, hipStream_t st) {
-  const int rot = a.rotary / 2 / VEC + ((a.dim - a.rotary) / VEC + 1) / 2;
-  const int plain = (a.dim / VEC + 1) / 2;
+  const int rot = places<VEC>(a.dim, a.rotary), plain = places<VEC>(a.dim, 0);
   const int most = rot > plain ? rot : plain;
   int lanes_shift = 0;
-  while ((1 << lanes_shift) < most) ++lanes_shift;  // dim <= 512: at most 256
+  while ((1 << lanes_shift) < most) ++lanes_shift;  // dim <= 256: at most 128 lanes
   const int all = (a.q ? a.heads : 0) + 2 * a.kv_heads;
-  int tokens_shift = 0;  // whole tokens that fit the workgroup's head slots
-  while ((256 >> lanes_shift >> (tokens_shift + 1)) >= all) ++tokens_shift;
+  // the workgroup of 1 to 4 waves whose slots are idle least, the larger of equals
+  int threads = 256, per_token = 256 >> lanes_shift, tokens_here = 1;
+  long best = -1;
+  for (int n = 64; n <= 256; n += 64) {
+    const int slots = n >> lanes_shift;
+    if (slots < 1) continue;
+    const int here = slots >= all ? slots / all : 1;
+    const int passes = (all + slots - 1) / slots;
+    const long busy = 4096L * here * all / ((long)slots * passes);
+    if (busy >= best) {
+      best = busy;
+      threads = n;
+      tokens_here = here;
+      per_token = here > 1 ? all : slots;
+    }
+  }
   const long tokens = a.batch * a.width;
-  const long blocks = (tokens + (1L << tokens_shift) - 1) >> tokens_shift;
-  hipLaunchKernelGGL((paged_append_k<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, a,
-                     lanes_shift, tokens_shift);
+  const long blocks = (tokens + tokens_here - 1) / tokens_here;
+  hipLaunchKernelGGL((paged_append_k<T, VEC>), dim3((unsigned)blocks), dim3(threads), 0, st, a,
+                     lanes_shift, per_token, tokens_here);
   return (int)hipGetLastError();
 }
 
