@@ -295,7 +295,14 @@ Tensor log_probs_raw(const Tensor& logits, const Tensor& tokens, double temperat
     *stats = torch::empty({tokens.numel(), 2}, f32);
     a.stats = stats->data_ptr<float>();
   }
-  if (a.rows) launched(launch_token_log_probs_fwd(&a, stream_of()), "token_log_probs");
+  if (!a.rows) return lp;
+  Tensor parts;
+  const int split = token_log_probs_parts(&a);
+  if (split > 1) {
+    parts = torch::empty({a.rows * split * 2}, f32);
+    a.parts = parts.data_ptr<float>();
+  }
+  launched(launch_token_log_probs_fwd(&a, stream_of()), "token_log_probs");
   return lp;
 }
 

@@ -28,9 +28,9 @@ struct TokenLogProbArgs {
   float inv_temperature;
   float* log_probs;     // [rows], forward
   float* stats;         // [rows][2]: the max and the sum of exp2; may be null in forward
+  float* parts;         // [rows][token_log_probs_parts()][2] where that is above 1, forward
   const float* upstream;  // [rows], backward
   void* grad;           // [rows][vocab] dense, backward
-  int stream_grad;      // the launcher's: write the gradient past the caches
 };
 
 // One operand of the policy loss seen as [rows][cols] with strides.
@@ -64,6 +64,7 @@ struct PolicyLossArgs {
 };
 
 extern "C" {
+int token_log_probs_parts(const TokenLogProbArgs* a);
 int launch_token_log_probs_fwd(const TokenLogProbArgs* a, void* stream);
 int launch_token_log_probs_bwd(const TokenLogProbArgs* a, void* stream);
 int policy_loss_blocks(long n);

@@ -72,15 +72,15 @@ __device__ __forceinline__ void load16<_Float16>(const _Float16* p, float (&x)[8
   for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
 }
 
-template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&x)[Vec16<T>::N], bool stream) {
+template <bool STREAM, typename T>
+__device__ __forceinline__ void store16(T* p, const float (&x)[Vec16<T>::N]) {
   typedef unsigned U4 __attribute__((ext_vector_type(4)));
   T h[Vec16<T>::N];
 #pragma unroll
   for (int i = 0; i < Vec16<T>::N; ++i) h[i] = (T)x[i];
   U4 u;
   __builtin_memcpy(&u, h, 16);
-  if (stream)
+  if (STREAM)
     __builtin_nontemporal_store(u, (U4*)p);
   else
     *(U4*)p = u;
@@ -124,7 +124,34 @@ __device__ __forceinline__ long token_at(const TokenLogProbArgs& a, long n) {
   return a.tokens_i32 ? (long)((const int*)a.tokens)[n] : ((const long*)a.tokens)[n];
 }
 
-// TPR threads share a row; BLOCK / TPR rows share a workgroup.
+// The row's log-prob and statistics from its joined (max, sum).
+template <typename T>
+__device__ __forceinline__ void write_row(const TokenLogProbArgs& a, long n, long tok, const T* row,
+                                          MaxSum r) {
+  float lp = 0.f, s = 1.f;
+  if (tok != a.ignore_index) {
+    // a row of -inf alone has no distribution: NaN, as 0 / 0
+    s = r.s == 0.f ? NAN : r.s;
+    lp = tok >= 0 && tok < a.vocab
+             ? fmaf((float)row[tok] - r.m, a.inv_temperature, -__builtin_amdgcn_logf(s) * kLn2)
+             : NAN;
+  } else {
+    r.m = 0.f;
+  }
+  a.log_probs[n] = lp;
+  if (a.stats) {
+    a.stats[2 * n] = r.m;
+    a.stats[2 * n + 1] = s;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_at(const TokenLogProbArgs& a, long n) {
+  return (const T*)a.logits + (n / a.width) * a.stride_batch + (n % a.width) * a.stride_row;
+}
+
+// TPR threads share a row; BLOCK / TPR rows share a workgroup, or with
+// gridDim.y > 1 that many workgroups share one row and leave their parts.
 template <typename T, int TPR, int BLOCK, int U>
 __global__ __launch_bounds__(BLOCK) void token_log_probs_fwd_k(const TokenLogProbArgs a) {
   constexpr int N = Vec16<T>::N;
@@ -136,48 +163,43 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_fwd_k(const TokenLogPro
     const long n = first + threadIdx.x / TPR;
     const bool live = n < a.rows;
     const long tok = live ? token_at(a, n) : a.ignore_index;
-    if (TPR > 64 ? tok == a.ignore_index : false) {  // the whole workgroup's row
-      if (t == 0) {
-        a.log_probs[n] = 0.f;
-        if (a.stats) {
-          a.stats[2 * n] = 0.f;
-          a.stats[2 * n + 1] = 1.f;
-        }
-      }
+    if (TPR > 64 && tok == a.ignore_index) {  // the whole workgroup's row
+      if (t == 0 && gridDim.y == 1) write_row<T>(a, n, tok, nullptr, {0.f, 1.f});
       continue;
     }
     MaxSum r = {-INFINITY, 0.f};
     const T* row = nullptr;
     if (tok != a.ignore_index) {
-      row = (const T*)a.logits + (n / a.width) * a.stride_batch + (n % a.width) * a.stride_row;
+      row = row_at<T>(a, n);
       const int mis = (int)(((size_t)row & 15) / sizeof(T));
       const int head = min(mis ? N - mis : 0, a.vocab);
       const int vecs = (a.vocab - head) / N;
       const int tail = a.vocab - head - vecs * N;
       const T* body = row + head;
       float edge[1][1];
-      if (t < head) {
+      if (t < head && blockIdx.y == 0) {
         edge[0][0] = (float)row[t];
         absorb<1, 1>(r, edge, c);
       }
-      if (TPR - 1 - t < tail) {
+      if (TPR - 1 - t < tail && blockIdx.y == gridDim.y - 1) {
         edge[0][0] = (float)row[a.vocab - (TPR - t)];
         absorb<1, 1>(r, edge, c);
       }
-      int v = t;
-      for (; v + (U - 1) * TPR < vecs; v += U * TPR) {
+      const int end = (int)((long)vecs * (blockIdx.y + 1) / gridDim.y);
+      int v = (int)((long)vecs * blockIdx.y / gridDim.y) + t;
+      for (; v + (U - 1) * TPR < end; v += U * TPR) {
         float x[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) load16<T>(body + (long)(v + u * TPR) * N, x[u]);
         absorb<U, N>(r, x, c);
       }
-      if (v < vecs) {  // what is left, all loads at once: the row's last vector for none
+      if (v < end) {  // what is left, all loads at once: the last vector again for none
         float x[U][N];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, vecs - 1) * N, x[u]);
+        for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, end - 1) * N, x[u]);
 #pragma unroll
         for (int u = 1; u < U; ++u)
-          if (v + u * TPR >= vecs)
+          if (v + u * TPR >= end)
 #pragma unroll
             for (int i = 0; i < N; ++i) x[u][i] = -INFINITY;
         absorb<U, N>(r, x, c);
@@ -196,24 +218,34 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_fwd_k(const TokenLogPro
       __syncthreads();  // part is written again for the next row
     }
     if (t == 0 && live) {
-      float lp = 0.f, s = 1.f;
-      if (tok != a.ignore_index) {
-        // a row of -inf alone has no distribution: NaN, as 0 / 0
-        s = r.s == 0.f ? NAN : r.s;
-        lp = tok >= 0 && tok < a.vocab
-                 ? fmaf((float)row[tok] - r.m, a.inv_temperature, -__builtin_amdgcn_logf(s) * kLn2)
-                 : NAN;
-      }
-      a.log_probs[n] = lp;
-      if (a.stats) {
-        a.stats[2 * n] = r.m;
-        a.stats[2 * n + 1] = s;
+      if (gridDim.y == 1) {
+        write_row<T>(a, n, tok, row, r);
+      } else {
+        a.parts[2 * (n * gridDim.y + blockIdx.y)] = r.m;
+        a.parts[2 * (n * gridDim.y + blockIdx.y) + 1] = r.s;
       }
     }
   }
 }
 
-template <typename T, int TPR, int BLOCK, int U>
+// A wave joins the parts of a row, in order.
+template <typename T>
+__global__ __launch_bounds__(64) void token_log_probs_join_k(const TokenLogProbArgs a, int parts) {
+  const long n = blockIdx.x;
+  const long tok = token_at(a, n);
+  const float c = a.inv_temperature * kLog2e;
+  MaxSum r = {-INFINITY, 0.f};
+  if (tok != a.ignore_index && (int)threadIdx.x < parts)
+    r = {a.parts[2 * (n * parts + threadIdx.x)], a.parts[2 * (n * parts + threadIdx.x) + 1]};
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    MaxSum o = {__shfl_xor(r.m, off, 64), __shfl_xor(r.s, off, 64)};
+    r = join(r, o, c);
+  }
+  if (threadIdx.x == 0) write_row<T>(a, n, tok, row_at<T>(a, n), r);
+}
+
+template <typename T, int TPR, int BLOCK, int U, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogProbArgs a) {
   constexpr int N = Vec16<T>::N;
   constexpr int ROWS = BLOCK / TPR;
@@ -226,18 +258,23 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
     const long tok = token_at(a, n);
     const float g = tok == a.ignore_index ? 0.f : a.upstream[n] * a.inv_temperature;
     T* out = (T*)a.grad + n * a.vocab;
-    const T* row = (const T*)a.logits + (n / a.width) * a.stride_batch + (n % a.width) * a.stride_row;
+    const T* row = row_at<T>(a, n);
     // aligned to the row that is written; reads may be unaligned
     const int mis = (int)(((size_t)out & 15) / sizeof(T));
     const int head = min(mis ? N - mis : 0, a.vocab);
     const int vecs = (a.vocab - head) / N;
     const int tail = a.vocab - head - vecs * N;
     T* obody = out + head;
+    // gridDim.y workgroups take a share of the row each
+    const bool has_head = t < head && blockIdx.y == 0;
+    const bool has_tail = TPR - 1 - t < tail && blockIdx.y == gridDim.y - 1;
+    const int end = (int)((long)vecs * (blockIdx.y + 1) / gridDim.y);
+    int v = (int)((long)vecs * blockIdx.y / gridDim.y) + t;
     if (g == 0.f) {  // a masked token: exact zeros, and its logits are not read
       const float zero[N] = {};
-      if (t < head) out[t] = (T)0.f;
-      if (TPR - 1 - t < tail) out[a.vocab - (TPR - t)] = (T)0.f;
-      for (int v = t; v < vecs; v += TPR) store16<T>(obody + (long)v * N, zero, a.stream_grad);
+      if (has_head) out[t] = (T)0.f;
+      if (has_tail) out[a.vocab - (TPR - t)] = (T)0.f;
+      for (; v < end; v += TPR) store16<STREAM, T>(obody + (long)v * N, zero);
       continue;
     }
     const bool known = tok >= 0 && tok < a.vocab;
@@ -248,8 +285,8 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
       const float d = scale * exp2_hw(((float)row[j] - m) * c);
       out[j] = (T)(j == tok ? d + g : d);
     };
-    if (t < head) one(t);
-    if (TPR - 1 - t < tail) one(a.vocab - (TPR - t));
+    if (has_head) one(t);
+    if (has_tail) one(a.vocab - (TPR - t));
     const long hot = tok - head;  // the token's place in the body
     auto finish = [&](int v, float (&x)[N]) {
 #pragma unroll
@@ -260,39 +297,64 @@ __global__ __launch_bounds__(BLOCK) void token_log_probs_bwd_k(const TokenLogPro
         for (int i = 0; i < N; ++i)
           if (i == at) x[i] += g;
       }
-      store16<T>(obody + (long)v * N, x, a.stream_grad);
+      store16<STREAM, T>(obody + (long)v * N, x);
     };
-    int v = t;
-    for (; v + (U - 1) * TPR < vecs; v += U * TPR) {
+    for (; v + (U - 1) * TPR < end; v += U * TPR) {
       float x[U][N];
 #pragma unroll
       for (int u = 0; u < U; ++u) load16<T>(body + (long)(v + u * TPR) * N, x[u]);
 #pragma unroll
       for (int u = 0; u < U; ++u) finish(v + u * TPR, x[u]);
     }
-    if (v < vecs) {  // what is left, all loads at once
+    if (v < end) {  // what is left, all loads at once
       float x[U][N];
 #pragma unroll
-      for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, vecs - 1) * N, x[u]);
+      for (int u = 0; u < U; ++u) load16<T>(body + (long)min(v + u * TPR, end - 1) * N, x[u]);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v + u * TPR < vecs) finish(v + u * TPR, x[u]);
+        if (v + u * TPR < end) finish(v + u * TPR, x[u]);
     }
   }
 }
 
 constexpr long kMaxBlocks = 1 << 20;
 
+// A gradient that the last-level cache (256 MB) cannot hold next to its logits is
+// written past it: what it would push out is what the passes around it read, and
+// its own reader finds it in memory either way.  (A variant of the kernel, not a
+// branch: the compiler joins the two stores into an ordinary one.)
+constexpr long kStreamBytes = 128L << 20;
+
 template <typename T, int TPR, int BLOCK, int U>
-int log_probs_launch(const TokenLogProbArgs& a, bool bwd, hipStream_t st) {
+int log_probs_fwd(const TokenLogProbArgs& a, int parts, hipStream_t st) {
   const long rows = BLOCK / TPR;
   const long need = (a.rows + rows - 1) / rows;
-  const dim3 grid((unsigned)(need < kMaxBlocks ? need : kMaxBlocks));
-  if (bwd)
-    hipLaunchKernelGGL((token_log_probs_bwd_k<T, TPR, BLOCK, U>), grid, dim3(BLOCK), 0, st, a);
-  else
-    hipLaunchKernelGGL((token_log_probs_fwd_k<T, TPR, BLOCK, U>), grid, dim3(BLOCK), 0, st, a);
+  const dim3 grid((unsigned)(need < kMaxBlocks ? need : kMaxBlocks), parts);
+  hipLaunchKernelGGL((token_log_probs_fwd_k<T, TPR, BLOCK, U>), grid, dim3(BLOCK), 0, st, a);
+  if (parts > 1)
+    hipLaunchKernelGGL((token_log_probs_join_k<T>), dim3((unsigned)a.rows), dim3(64), 0, st, a, parts);
   return (int)hipGetLastError();
+}
+
+template <typename T, int TPR, int BLOCK, int U>
+int log_probs_bwd(const TokenLogProbArgs& a, int parts, hipStream_t st) {
+  const long rows = BLOCK / TPR;
+  const long need = (a.rows + rows - 1) / rows;
+  const dim3 grid((unsigned)(need < kMaxBlocks ? need : kMaxBlocks), parts);
+  if (a.rows * a.vocab * (long)sizeof(T) > kStreamBytes)
+    hipLaunchKernelGGL((token_log_probs_bwd_k<T, TPR, BLOCK, U, true>), grid, dim3(BLOCK), 0, st, a);
+  else
+    hipLaunchKernelGGL((token_log_probs_bwd_k<T, TPR, BLOCK, U, false>), grid, dim3(BLOCK), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+// Workgroups to a long row where rows are few: as many as give every CU one, with
+// 16 KB each at least (bf16, 1 / 8 / 64 rows of 100 KB, backward: 7.8 / 8.1 / 8.8 us
+// with one, 6.3 / 6.3 / 7.2 shared; twice as many workgroups 6.3 / 6.3 / 9.1).
+int shares_of_row(long bytes, long rows) {
+  const long share = bytes / 16384, fill = 256 / rows;
+  const long n = share < fill ? share : fill;
+  return n < 1 ? 1 : n < 64 ? (int)n : 64;
 }
 
 // Threads to a row, by the row's bytes (MI355X, bf16, 8192 rows, forward /
@@ -309,10 +371,11 @@ template <typename T>
 int log_probs_dispatch(const TokenLogProbArgs& a, bool bwd, hipStream_t st) {
   const long bytes = (long)a.vocab * (long)sizeof(T);
   if (bytes <= 4096 || (bytes <= 8192 && a.rows >= 1024))
-    return log_probs_launch<T, 64, 256, 8>(a, bwd, st);
-  if (bytes <= 40960) return log_probs_launch<T, 256, 256, 4>(a, bwd, st);
-  return bwd ? log_probs_launch<T, 1024, 1024, 4>(a, bwd, st)
-             : log_probs_launch<T, 512, 512, 4>(a, bwd, st);
+    return bwd ? log_probs_bwd<T, 64, 256, 8>(a, 1, st) : log_probs_fwd<T, 64, 256, 8>(a, 1, st);
+  if (bytes <= 40960)
+    return bwd ? log_probs_bwd<T, 256, 256, 4>(a, 1, st) : log_probs_fwd<T, 256, 256, 4>(a, 1, st);
+  if (!bwd) return log_probs_fwd<T, 512, 512, 4>(a, a.parts ? token_log_probs_parts(&a) : 1, st);
+  return log_probs_bwd<T, 1024, 1024, 4>(a, shares_of_row(bytes, a.rows), st);
 }
 
 int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
@@ -715,18 +778,23 @@ void policy_fwd_block(const PolicyLossArgs& a, bool dense, hipStream_t st) {
 
 }  // namespace
 
+// Workgroups that share a row forward.  A second launch joins them, so only rows
+// long enough to pay for it are split (bf16, 8 / 64 rows, one workgroup each ->
+// shared and joined, us): 100 KB 8.8 / 9.0 -> 9.3 / 9.9, 160 KB 10.4 / 10.7 ->
+// 9.3 / 10.6, 256 KB 12.4 / 12.7 -> 9.3 / 11.0, 320 KB 14.1 / 14.5 -> 9.2 / 11.4; the
+// second launch also takes the host 2 us.
+extern "C" int token_log_probs_parts(const TokenLogProbArgs* a) {
+  const long bytes = (long)a->vocab * (a->dtype == RL_F32 ? 4 : 2);
+  if (bytes <= (192L << 10) || a->rows > 64 || a->rows < 1) return 1;
+  return shares_of_row(bytes, a->rows);
+}
+
 extern "C" int launch_token_log_probs_fwd(const TokenLogProbArgs* a, void* stream) {
   return log_probs_any(a, false, stream);
 }
 
-// A gradient that the last-level cache (256 MB) cannot hold next to its logits is
-// written past it: what it would push out is what the passes around it read, and
-// its own reader finds it in memory either way.  2048 x 50257 bf16 (206 MB),
-// forward + backward: 57 + 73 -> 42 + 69 us; 8192 rows: 172 + 276 -> 144 + 279.
-extern "C" int launch_token_log_probs_bwd(const TokenLogProbArgs* args, void* stream) {
-  TokenLogProbArgs a = *args;
-  a.stream_grad = a.rows * a.vocab * (a.dtype == RL_F32 ? 4 : 2) > (128L << 20);
-  return log_probs_any(&a, true, stream);
+extern "C" int launch_token_log_probs_bwd(const TokenLogProbArgs* a, void* stream) {
+  return log_probs_any(a, true, stream);
 }
 
 extern "C" int policy_loss_blocks(long n) {

@@ -66,7 +66,8 @@ def log_probs_tolerance(z, g, p, grad, vocab, dtype):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 7), (4, 8), (2, 503), (3, 4097), (2, 50257), (1030, 2049)])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 7), (4, 8), (2, 503), (3, 4097), (2, 50257), (1030, 2049),
+                                   (1, 130001), (60, 100003), (65, 100003)])
 @pytest.mark.parametrize("temperature", [1.0, 0.7])
 def test_log_probs_and_gradient(device, dtype, shape, temperature):
     rows, vocab = shape
