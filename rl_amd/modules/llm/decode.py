@@ -23,15 +23,35 @@ tests/test_llm_bench.py (same sampling distribution as
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn.functional as F
 
-__all__ = ["GraphedGPT2Decoder"]
+from ... import ops
+from ...tensordict import TensorDict
+from .paged_cache import PagedKVCache
+
+__all__ = ["GraphedGPT2Decoder", "PagedGPT2Decoder"]
 
 
 class GraphedGPT2Decoder:
     def __init__(self, model, batch: int, max_len: int, device,
                  dtype=torch.bfloat16):
+        self._bind(model, batch, max_len, device, dtype)
+        # static KV + bookkeeping buffers
+        kv = (self.L, self.B, self.nh, self.T, self.dh)
+        self.K = torch.zeros(kv, device=device, dtype=dtype)
+        self.Vv = torch.zeros(kv, device=device, dtype=dtype)
+        self.mask = torch.full((self.T,), float("-inf"), device=device)
+        self.cur = torch.zeros(self.B, 1, dtype=torch.long, device=device)
+        self.pos = torch.zeros(1, dtype=torch.long, device=device)
+        self.pos_out = torch.zeros(1, dtype=torch.long, device=device)
+        self.gen_buf = torch.zeros(self.B, self.T, dtype=torch.long,
+                                   device=device)
+        self._graph = None
+
+    def _bind(self, model, batch, max_len, device, dtype) -> None:
         self.model = model
         self.cfg = model.config
         self.B = batch
@@ -48,17 +68,6 @@ class GraphedGPT2Decoder:
         # bf16 weight caches (refreshed per training iteration)
         self._w = {}
         self.refresh_weights()
-        # static KV + bookkeeping buffers
-        kv = (self.L, self.B, self.nh, self.T, self.dh)
-        self.K = torch.zeros(kv, device=device, dtype=dtype)
-        self.Vv = torch.zeros(kv, device=device, dtype=dtype)
-        self.mask = torch.full((self.T,), float("-inf"), device=device)
-        self.cur = torch.zeros(self.B, 1, dtype=torch.long, device=device)
-        self.pos = torch.zeros(1, dtype=torch.long, device=device)
-        self.pos_out = torch.zeros(1, dtype=torch.long, device=device)
-        self.gen_buf = torch.zeros(self.B, self.T, dtype=torch.long,
-                                   device=device)
-        self._graph = None
 
     # ------------------------------------------------------------------ #
     def refresh_weights(self) -> None:
@@ -200,4 +209,158 @@ class GraphedGPT2Decoder:
                     self._decode_body()
         return torch.cat(
             [prompts, self.gen_buf[:, :gen_tokens]], dim=1
+        )
+
+
+class PagedGPT2Decoder(GraphedGPT2Decoder):
+    """GPT-2 decode over a :class:`PagedKVCache`: prompts of any lengths in
+    one batch, an optional end token, and the behavior log-probs that the
+    policy losses need, recorded while sampling.
+
+    Per generated token and layer: one cache append
+    (:func:`rl_amd.ops.paged_kv_append`) and one attention over each
+    sequence's own length (:func:`rl_amd.ops.paged_attention_decode`), where
+    :class:`GraphedGPT2Decoder` attends over ``max_len`` for every sequence.
+    After :meth:`capture` each token is one graph replay; a sequence that has
+    produced ``eos_token_id`` stops writing to its cache.
+
+    Args:
+        model: a transformers GPT-2 with LM head.
+        batch: sequences per rollout.
+        max_len: longest prompt plus response; at most the model's positions.
+        temperature: of the sampling and of the recorded log-probs.
+        eos_token_id: stop a sequence after this token; None: never.
+        page_size: positions per cache page (a power of two).
+    """
+
+    def __init__(self, model, batch: int, max_len: int, device, dtype=torch.bfloat16, *,
+                 temperature: float = 1.0, eos_token_id: Optional[int] = None, page_size: int = 16):
+        if max_len > model.config.n_positions:
+            raise ValueError(
+                f"PagedGPT2Decoder: max_len {max_len} exceeds the model's {model.config.n_positions} positions")
+        self._bind(model, batch, max_len, device, dtype)
+        self.temperature = temperature
+        self.eos_token_id = eos_token_id
+        self.cache = PagedKVCache(
+            self.L, batch * -(-max_len // page_size), self.nh, self.dh, batch=batch,
+            max_length=max_len, page_size=page_size, dtype=dtype, device=device)
+        self.cur = torch.zeros(batch, dtype=torch.long, device=device)
+        self.active = torch.ones(batch, dtype=torch.int32, device=device)
+        self.pos_out = torch.zeros(1, dtype=torch.long, device=device)
+        self.gen_buf = torch.zeros(batch, max_len, dtype=torch.long, device=device)
+        self.lp_buf = torch.zeros(batch, max_len, dtype=torch.float32, device=device)
+        self.mask_buf = torch.zeros(batch, max_len, dtype=torch.bool, device=device)
+        self._graph = None
+
+    def _step_logits(self) -> torch.Tensor:
+        """One decode forward: ``[B, V]`` fp32 logits after the tokens in
+        ``self.cur``, whose keys and values join the cache."""
+        w, eps, dt = self._w, self.cfg.layer_norm_epsilon, self.dtype
+        B, nh, dh, E = self.B, self.nh, self.dh, self.E
+        cache = self.cache
+        cache.extend(self.active)
+        x = (w["wte"].index_select(0, self.cur)
+             + w["wpe"].index_select(0, cache.start.clamp(max=self.T - 1)))
+
+        def norm(x, name):
+            return F.layer_norm(x.float(), (E,), w[f"{name[0]}_w{name[1]}"],
+                                w[f"{name[0]}_b{name[1]}"], eps).to(dt)
+
+        for i in range(self.L):
+            qkv = torch.addmm(w[f"attn_b{i}"], norm(x, ("ln1", i)), w[f"attn_w{i}"])
+            q, k, v = (t.view(B, 1, nh, dh) for t in qkv.split(E, dim=-1))
+            cache.append(i, k, v, lengths=self.active)
+            o = cache.attend(i, q[:, 0]).view(B, E)
+            x = x + torch.addmm(w[f"proj_b{i}"], o, w[f"proj_w{i}"])
+            h = torch.addmm(w[f"fc_b{i}"], norm(x, ("ln2", i)), w[f"fc_w{i}"])
+            h = F.gelu(h, approximate="tanh")
+            x = x + torch.addmm(w[f"fc2_b{i}"], h, w[f"fc2_w{i}"])
+        xn = F.layer_norm(x.float(), (E,), w["lnf_w"], w["lnf_b"], eps)
+        return torch.matmul(xn.to(dt), w["wte"].t()).float()
+
+    def _sample(self, logits: torch.Tensor) -> None:
+        """Sample the next token of every sequence and record it; stopped
+        sequences record the end token outside the mask."""
+        on = self.active.bool()
+        nxt = torch.multinomial(torch.softmax(logits / self.temperature, -1), 1).squeeze(-1)
+        if self.eos_token_id is not None:
+            nxt = torch.where(on, nxt, self.eos_token_id)
+        lp = ops.token_log_probs(logits, torch.where(on, nxt, -100), temperature=self.temperature)
+        self.gen_buf.index_copy_(1, self.pos_out, nxt[:, None])
+        self.lp_buf.index_copy_(1, self.pos_out, lp[:, None])
+        self.mask_buf.index_copy_(1, self.pos_out, on[:, None])
+        self.cur.copy_(nxt)
+        if self.eos_token_id is not None:
+            self.active.mul_(nxt != self.eos_token_id)
+        self.pos_out.add_(1)
+
+    def _decode_body(self) -> None:
+        self._sample(self._step_logits())
+
+    def capture(self) -> bool:
+        # its warm-up decodes three tokens past the first
+        return self.T >= 4 and super().capture()
+
+    def prefill(self, prompts: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> None:
+        """HF forward over right-padded ``prompts [B, P]``; fills the cache
+        with each sequence's first ``lengths`` positions (default: all) and
+        samples the first response token."""
+        B, P = prompts.shape
+        if B != self.B or not 0 < P <= self.T:
+            raise ValueError(f"PagedGPT2Decoder: prompts must be [{self.B}, up to {self.T}], got {list(prompts.shape)}")
+        if lengths is None:
+            lengths = torch.full((B,), P, dtype=torch.long)
+        host = lengths.tolist()
+        if len(host) != B or min(host) < 1 or max(host) > P:
+            raise ValueError(f"PagedGPT2Decoder: lengths must hold {B} numbers from 1 to {P}, got {host}")
+        self.cache.reset()
+        self.cache.reserve([self.T] * B)
+        count = lengths.to(device=self.device, dtype=torch.int32)
+        with torch.no_grad(), torch.autocast(
+            "cuda", dtype=self.dtype, cache_enabled=False, enabled=prompts.is_cuda,
+        ):
+            out = self._tr(input_ids=prompts, use_cache=True)
+            last = out.last_hidden_state[torch.arange(B, device=prompts.device), count.long() - 1]
+            logits = self.model.lm_head(last).float()
+        past = out.past_key_values
+        self.cache.extend(count)
+        with torch.no_grad():
+            for i in range(self.L):
+                if hasattr(past, "layers"):  # transformers >= 4.54 Cache
+                    k, v = past.layers[i].keys, past.layers[i].values
+                elif hasattr(past, "key_cache"):
+                    k, v = past.key_cache[i], past.value_cache[i]
+                else:
+                    k, v = past[i]
+                self.cache.append(i, k.transpose(1, 2).to(self.dtype),
+                                  v.transpose(1, 2).to(self.dtype), lengths=count)
+            self.active.fill_(1)
+            self.mask_buf.fill_(False)
+            self.lp_buf.zero_()
+            self.pos_out.zero_()
+            self._sample(logits)
+
+    def rollout(self, prompts: torch.Tensor, gen_tokens: int,
+                lengths: Optional[torch.Tensor] = None) -> TensorDict:
+        """Generate up to ``gen_tokens`` tokens for each prompt.  Returns the
+        keys the policy losses read: ``tokens_response``, ``log_probs`` (of
+        the sampling distribution) and ``attention_mask_response``, all
+        ``[B, gen_tokens]``."""
+        if gen_tokens < 1 or prompts.shape[1] + gen_tokens > self.T:
+            raise ValueError(
+                f"PagedGPT2Decoder: {prompts.shape[1]} prompt and {gen_tokens} new tokens do not fit max_len {self.T}")
+        self.prefill(prompts, lengths)
+        with torch.no_grad():
+            for _ in range(gen_tokens - 1):
+                if self._graph is not None:
+                    self._graph.replay()
+                else:
+                    self._decode_body()
+        return TensorDict(
+            {
+                "tokens_response": self.gen_buf[:, :gen_tokens].clone(),
+                "log_probs": self.lp_buf[:, :gen_tokens].clone(),
+                "attention_mask_response": self.mask_buf[:, :gen_tokens].clone(),
+            },
+            batch_size=[self.B],
         )

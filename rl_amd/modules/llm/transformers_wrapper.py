@@ -12,10 +12,18 @@ from typing import Any, List, Optional, Sequence, Union
 
 import torch
 
+from ... import ops
 from ...data.llm.history import History
 from ...tensordict import NonTensorData, TensorDict, TensorDictBase, TensorDictModuleBase
 
 __all__ = ["LLMWrapperBase", "TransformersWrapper"]
+
+
+def _log_probs_of(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+    """``log_softmax(logits)`` at ``tokens``, in the logits' dtype."""
+    if logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        return ops.token_log_probs(logits, tokens).to(logits.dtype)
+    return logits.log_softmax(-1).gather(-1, tokens.unsqueeze(-1)).squeeze(-1)
 
 
 class LLMWrapperBase(TensorDictModuleBase):
@@ -119,9 +127,7 @@ class TransformersWrapper(LLMWrapperBase):
         # per-step log-probs of the sampled tokens
         lps = []
         for t, scores in enumerate(out.scores):
-            logp = scores.log_softmax(-1)
-            tok = resp_tokens[:, t]
-            lps.append(logp.gather(-1, tok.unsqueeze(-1)).squeeze(-1))
+            lps.append(_log_probs_of(scores, resp_tokens[:, t]))
         log_probs = torch.stack(lps, 1) if lps else torch.zeros_like(resp_tokens, dtype=torch.float)
         resp_texts = self.tokenizer.batch_decode(resp_tokens, skip_special_tokens=True)
         td.set_non_tensor("text_response", resp_texts if len(td.batch_size) else resp_texts[0])
@@ -162,8 +168,7 @@ class TransformersWrapper(LLMWrapperBase):
         logits = self.model(input_ids=full, attention_mask=full_mask).logits
         # logits at position t predict token t+1
         resp_logits = logits[:, ids.shape[1] - 1 : -1]
-        logp = resp_logits.log_softmax(-1)
-        lp = logp.gather(-1, resp.unsqueeze(-1)).squeeze(-1)
+        lp = _log_probs_of(resp_logits, resp)
         td.set("log_probs", lp if td.device is None else lp.to(td.device or lp.device))
         return td
 

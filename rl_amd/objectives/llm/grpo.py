@@ -10,6 +10,7 @@ from typing import Optional
 
 import torch
 
+from ... import ops
 from ...tensordict import TensorDict, TensorDictBase, TensorDictModuleBase
 from ..common import LossModule
 
@@ -82,6 +83,59 @@ class GRPOLoss(LossModule):
         g2 = ratio.clamp(1 - self.clip_epsilon, 1 + self.clip_epsilon) * adv
         return torch.minimum(g1, g2), ratio
 
+    # (variant, low, high) of ops.token_policy_loss that equals _ratio_clip_gain
+    def _fused_clip(self):
+        return "clip", self.clip_epsilon, self.clip_epsilon
+
+    @staticmethod
+    def _broadcasts(x, to) -> bool:
+        return x.dim() <= to.dim() and all(
+            a in (1, b) for a, b in zip(reversed(x.shape), reversed(to.shape)))
+
+    def _fused(self, new_lp, old_lp, adv, mask, ref_lp) -> Optional[TensorDictBase]:
+        """The losses from one kernel, or None where it does not apply: off
+        the GPU, for a subclass with a gain or reduction of its own, for
+        operands that broadcast or carry gradients themselves."""
+        owner = next(c for c in type(self).__mro__ if "_ratio_clip_gain" in c.__dict__)
+        data = [t for t in (old_lp, adv, mask, ref_lp) if t is not None]
+        same = [t for t in (old_lp, mask, ref_lp) if t is not None]
+        if (
+            not new_lp.is_cuda
+            or "_fused_clip" not in owner.__dict__
+            or type(self)._reduce is not GRPOLoss._reduce
+            or new_lp.numel() == 0
+            or any(t.device != new_lp.device or t.requires_grad for t in data)
+            or any(t.shape != new_lp.shape for t in same)
+            or not self._broadcasts(adv, new_lp)
+            or any(t.dtype not in (torch.float32, torch.bfloat16, torch.float16)
+                   for t in (new_lp, old_lp, adv) + (() if ref_lp is None else (ref_lp,)))
+            or (mask is not None and mask.is_complex())
+        ):
+            return None
+        variant, low, high = self._fused_clip()
+        if not all(isinstance(x, (int, float)) and x >= 0 for x in (low, high)):
+            return None
+        loss = ops.token_policy_loss(
+            new_lp, old_lp, adv, mask, ref_lp, clip_low=low, clip_high=high, variant=variant,
+            kl_coeff=self.kl_to_ref_coeff if ref_lp is not None else 0.0,
+            entropy_coeff=self.entropy_coeff or 0.0,
+            reduction="mean" if self.reduction == "mean" else "sum")
+        dtype = new_lp.dtype
+        out = TensorDict(
+            {
+                "loss_objective": loss.loss_objective.to(dtype),
+                "clip_fraction": loss.clip_fraction,
+                "ESS": loss.ess.to(dtype),
+            },
+            batch_size=[],
+        )
+        if ref_lp is not None:
+            out.set("loss_kl_to_ref", loss.loss_kl.to(dtype))
+            out.set("kl_to_ref", loss.kl.to(dtype))
+        if self.entropy_coeff:
+            out.set("loss_entropy", loss.loss_entropy.to(dtype))
+        return out
+
     def forward(self, tensordict: TensorDictBase) -> TensorDictBase:
         keys = self.tensor_keys
         td = tensordict.clone(False)
@@ -93,9 +147,15 @@ class GRPOLoss(LossModule):
         self.actor_network.generate = False
         new_td = self.actor_network(td.clone(False))
         new_lp = new_td.get(keys.sample_log_prob)
+        mask = td.get(keys.mask, None)
+        ref_lp = None
+        if self.kl_to_ref_coeff is not None:
+            ref_lp = td.get(keys.ref_log_prob, None)
+        fused = self._fused(new_lp, old_lp.detach(), adv, mask, ref_lp)
+        if fused is not None:
+            return fused
         log_w = new_lp - old_lp.detach()
         gain, ratio = self._ratio_clip_gain(log_w, adv)
-        mask = td.get(keys.mask, None)
         if mask is None:
             resp = td.get("tokens_response", None)
             if resp is not None:
@@ -108,14 +168,12 @@ class GRPOLoss(LossModule):
             },
             batch_size=[],
         )
-        if self.kl_to_ref_coeff is not None:
-            ref_lp = td.get(keys.ref_log_prob, None)
-            if ref_lp is not None:
-                # unbiased k3 estimator (Schulman)
-                lr = ref_lp - new_lp
-                kl = lr.exp() - 1 - lr
-                out.set("loss_kl_to_ref", self.kl_to_ref_coeff * self._reduce(kl, mask))
-                out.set("kl_to_ref", self._reduce(kl.detach(), mask))
+        if ref_lp is not None:
+            # unbiased k3 estimator (Schulman)
+            lr = ref_lp - new_lp
+            kl = lr.exp() - 1 - lr
+            out.set("loss_kl_to_ref", self.kl_to_ref_coeff * self._reduce(kl, mask))
+            out.set("kl_to_ref", self._reduce(kl.detach(), mask))
         if self.entropy_coeff:
             ent = -new_lp
             out.set("loss_entropy", -self.entropy_coeff * self._reduce(ent, mask))
@@ -130,6 +188,9 @@ class DAPO(GRPOLoss):
         super().__init__(actor_network, clip_epsilon=clip_epsilon_low, **kwargs)
         self.clip_epsilon_high = clip_epsilon_high
 
+    def _fused_clip(self):
+        return "clip", self.clip_epsilon, self.clip_epsilon_high
+
     def _ratio_clip_gain(self, log_w, adv):
         ratio = log_w.exp()
         g1 = ratio * adv
@@ -140,6 +201,9 @@ class DAPO(GRPOLoss):
 class CISPOLoss(GRPOLoss):
     """Clipped-importance-sampling PG (reference grpo.py:1004): clip the
     IS weight itself, keep the gradient through log-probs."""
+
+    def _fused_clip(self):
+        return "cispo", self.clip_epsilon, self.clip_epsilon
 
     def _ratio_clip_gain(self, log_w, adv):
         ratio = log_w.exp()

@@ -1,0 +1,517 @@
+"""The language-model operators as the framework uses them: the paged GPT-2
+rollout, the wrappers and the GRPO family; streams, graphs and far offsets."""
+import gc
+import math
+
+import pytest
+import torch
+
+from rl_amd import ops
+from rl_amd.modules.llm import PagedKVCache
+from rl_amd.objectives import GRPOLoss
+from rl_amd.objectives.llm import CISPOLoss, DAPO
+from rl_amd.tensordict import TensorDict, TensorDictModuleBase
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24
+
+
+def make_lm(seed=0, **kw):
+    transformers = pytest.importorskip("transformers")
+    torch.manual_seed(seed)
+    cfg = transformers.GPT2Config(**{**dict(
+        n_layer=2, n_head=4, n_embd=128, vocab_size=503, n_positions=64,
+        resid_pdrop=0.0, embd_pdrop=0.0, attn_pdrop=0.0), **kw})
+    return transformers.GPT2LMHeadModel(cfg).eval()
+
+
+class Actor(TensorDictModuleBase):
+    """Log-probs of the response over the whole sequence's logits: prompt and
+    padding are ignored places, nothing is sliced or copied."""
+
+    def __init__(self, model, plain=False):
+        super().__init__()
+        self.model = model
+        self.plain = plain
+        self.in_keys, self.out_keys = ["ids", "targets"], ["log_probs"]
+
+    def forward(self, td):
+        logits = self.model(input_ids=td.get("ids")).logits
+        targets = td.get("targets")
+        if self.plain:
+            at = targets.clamp(min=0).unsqueeze(-1)
+            lp = logits.log_softmax(-1).gather(-1, at).squeeze(-1)
+            lp = torch.where(targets == -100, 0.0, lp)
+        else:
+            lp = ops.token_log_probs(logits, targets)
+        td.set("log_probs", lp)
+        return td
+
+
+# --------------------------------------------------------------------------- #
+# the cache
+# --------------------------------------------------------------------------- #
+def test_cache_pages():
+    cache = PagedKVCache(2, 5, 1, 8, batch=2, max_length=40, page_size=16, dtype=torch.float32)
+    cache.reserve([17, 16])
+    assert cache.free_pages == 2
+    held = cache.page_table[cache.page_table >= 0].tolist()
+    assert len(set(held)) == 3 and cache.page_table.shape == (2, 3)
+    cache.reserve([17, 0])
+    assert cache.free_pages == 2
+    with pytest.raises(RuntimeError, match="pages needed"):
+        cache.reserve([40, 40])
+    assert cache.free_pages == 2
+    with pytest.raises(ValueError, match="max_length"):
+        cache.reserve([41, 0])
+    with pytest.raises(ValueError, match="lengths"):
+        cache.reserve([1])
+    cache.extend(torch.tensor([17, 3], dtype=torch.int32))
+    cache.release(0)
+    assert cache.free_pages == 4 and cache.lengths.tolist() == [0, 3]
+    assert (cache.page_table[0] == -1).all()
+    with pytest.raises(ValueError, match="power of two"):
+        PagedKVCache(1, 1, 1, 8, batch=1, max_length=4, page_size=12)
+    with pytest.raises(ValueError, match="at least 1"):
+        PagedKVCache(1, 0, 1, 8, batch=1, max_length=4)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_cache_steps_with_rotation(device, interleaved):
+    """Prompt and then single tokens through cache.append and cache.attend
+    against attention over everything in 64 bits; a sequence that pauses."""
+    g = torch.Generator().manual_seed(4)
+    batch, heads, kv_heads, dim, prompt, steps = 3, 6, 2, 64, 11, 9
+    n = prompt + steps
+    q, k, v = (torch.randn(batch, n, h, dim, generator=g) for h in (heads, kv_heads, kv_heads))
+    rope = ops.rotary_table(64, 32, device=device)
+    cache = PagedKVCache(1, 40, kv_heads, dim, batch=batch, max_length=n, page_size=4,
+                         dtype=torch.float32, device=device)
+    cache.reserve([n] * batch)
+    held = torch.tensor([11, 4, 1])
+    cache.extend(held.to(device, torch.int32))
+    cache.append(0, k[:, :prompt].to(device), v[:, :prompt].to(device), rope=rope,
+                 lengths=held.to(device), interleaved=interleaved)
+    seen = [[(k[b, t], v[b, t]) for t in range(held[b])] for b in range(batch)]
+    cos, sin = (t.cpu().double() for t in rope)
+
+    def turn(x, p):
+        x = x.double().clone()
+        one = slice(0, 32, 2) if interleaved else slice(0, 16)
+        two = slice(1, 32, 2) if interleaved else slice(16, 32)
+        a, b = x[..., one].clone(), x[..., two].clone()
+        x[..., one], x[..., two] = a * cos[p] - b * sin[p], b * cos[p] + a * sin[p]
+        return x
+
+    for t in range(prompt, n):
+        on = torch.tensor([1, 1, int(t % 3 == 0)], dtype=torch.int32)
+        cache.extend(on.to(device))
+        qr = cache.append(0, k[:, t:t + 1].to(device), v[:, t:t + 1].to(device), q=q[:, t:t + 1].to(device),
+                          rope=rope, lengths=on.to(device), interleaved=interleaved)
+        out = cache.attend(0, qr[:, 0]).cpu().double()
+        for b in range(batch):
+            if not on[b]:
+                continue
+            seen[b].append((k[b, t], v[b, t]))
+            keys = torch.stack([turn(x, p) for p, (x, _) in enumerate(seen[b])])
+            values = torch.stack([y for _, y in seen[b]]).double()
+            query = turn(q[b, t], len(seen[b]) - 1)
+            for h in range(heads):
+                key, value = keys[:, h // 3], values[:, h // 3]
+                p = torch.softmax(key @ query[h] / 8.0, 0)
+                # rotated operands are off by 4 u of their size, a score adds up
+                # dim products (2 u each), its error goes through exp; n sums
+                off = float((key.abs() @ query[h].abs()).max()) / 8.0 * U * (2 * dim + 16)
+                tol = (2 * off + 2 * U * (n + 16)) * (p @ value.abs()) + U * value.abs().max()
+                assert ((out[b, h] - p @ value).abs() <= tol).all()
+
+
+# --------------------------------------------------------------------------- #
+# the paged rollout
+# --------------------------------------------------------------------------- #
+def ragged_prompts(device, seed=1, batch=4, width=9):
+    g = torch.Generator().manual_seed(seed)
+    prompts = torch.randint(0, 503, (batch, width), generator=g).to(device)
+    return prompts, torch.tensor([9, 1, 4, 7])[:batch]
+
+
+def hf_log_probs(model, prompts, lengths, out, temperature):
+    """The response's log-probs by the model over each whole sequence."""
+    tokens, mask = out.get("tokens_response"), out.get("attention_mask_response")
+    want = torch.zeros(tokens.shape, dtype=torch.float64)
+    with torch.no_grad():
+        for b in range(len(lengths)):
+            n, m = int(lengths[b]), int(mask[b].sum())
+            ids = torch.cat([prompts[b, :n], tokens[b, :m]])[None]
+            lp = (model(ids).logits[0, n - 1:-1].double() / temperature).log_softmax(-1)
+            want[b, :m] = lp.gather(-1, tokens[b, :m, None]).squeeze(-1).cpu()
+    return want
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("graph", [False, True])
+def test_paged_rollout_records_the_models_log_probs(device, graph):
+    """fp32 decode of ragged prompts: the recorded log-probs are those of the
+    HF model on each sequence by itself.  Two fp32 forwards of two layers and
+    sums of up to 512 products differ by some 100 u of logits of size 1; 2e-4
+    is 30 times that."""
+    if graph and device == "cpu":
+        pytest.skip("graphs need a GPU")
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm().to(device)
+    dec = PagedGPT2Decoder(model, 4, 40, device, dtype=torch.float32, temperature=0.8, page_size=8)
+    prompts, lengths = ragged_prompts(device)
+    if graph:
+        dec.prefill(prompts, lengths)
+        assert dec.capture()
+    for seed in range(3 if graph else 1):
+        torch.manual_seed(seed)
+        prompts, lengths = ragged_prompts(device, seed)
+        out = dec.rollout(prompts, 20, lengths)
+        assert out.get("attention_mask_response").all()
+        want = hf_log_probs(model, prompts, lengths, out, 0.8)
+        assert (out.get("log_probs").cpu().double() - want).abs().max() < 2e-4
+        # eager work between the replays
+        gc.collect()
+        if device == "cuda":
+            torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_paged_rollout_stops_at_the_end_token(device):
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm(vocab_size=7).to(device)
+    dec = PagedGPT2Decoder(model, 4, 40, device, dtype=torch.float32, eos_token_id=3)
+    torch.manual_seed(5)
+    prompts, lengths = ragged_prompts(device)
+    prompts = prompts % 7
+    out = dec.rollout(prompts, 24, lengths)
+    tokens, lp, mask = (out.get(x).cpu() for x in ("tokens_response", "log_probs", "attention_mask_response"))
+    for b in range(4):
+        m = int(mask[b].sum())
+        assert mask[b, :m].all()
+        assert (tokens[b, : m - 1] != 3).all()
+        if m < 24:
+            assert tokens[b, m - 1] == 3 and (tokens[b, m:] == 3).all() and (lp[b, m:] == 0).all()
+        # the end token itself is sampled, not decoded: it never enters the cache
+        assert int(dec.cache.lengths[b]) == int(lengths[b]) + min(m - 1, 23)
+    assert (mask.sum(-1) < 24).any()
+    want = hf_log_probs(model, prompts, lengths, out, 1.0)
+    assert (lp.double() - want).abs().max() < 2e-4
+
+
+def test_paged_rollout_refusals():
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm()
+    with pytest.raises(ValueError, match="positions"):
+        PagedGPT2Decoder(model, 2, 65, "cpu")
+    dec = PagedGPT2Decoder(model, 2, 20, "cpu", dtype=torch.float32)
+    prompts = torch.zeros(2, 5, dtype=torch.long)
+    with pytest.raises(ValueError, match="do not fit"):
+        dec.rollout(prompts, 16)
+    with pytest.raises(ValueError, match="prompts must be"):
+        dec.rollout(prompts[:1], 4)
+    for bad in ([5], [0, 5], [5, 6]):
+        with pytest.raises(ValueError, match="lengths must"):
+            dec.rollout(prompts, 4, torch.tensor(bad))
+
+
+@pytest.mark.gpu
+def test_paged_rollout_matches_hf_bf16():
+    """bf16, mixed prompt lengths: the next-token logits of the HF model."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm(n_layer=4).cuda()
+    dec = PagedGPT2Decoder(model, 4, 32, "cuda")
+    prompts, lengths = ragged_prompts("cuda")
+    dec.prefill(prompts, lengths)
+    tok = dec.cur.clone()
+    with torch.no_grad():
+        logits = dec._step_logits()
+        for b in range(4):
+            ids = torch.cat([prompts[b, : int(lengths[b])], tok[b:b + 1]])[None]
+            with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+                ref = model(ids).logits[0, -1].float()
+            assert torch.allclose(logits[b], ref, atol=0.5, rtol=0.05)
+
+
+# --------------------------------------------------------------------------- #
+# rollout, log-probs and loss together
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("loss_cls", [GRPOLoss, DAPO, CISPOLoss])
+def test_grpo_step_over_the_operators(device, loss_cls):
+    """One RLHF step: paged rollout, log-probs over the full logits, loss with
+    its KL term, gradients of every weight; against the same step in plain
+    torch in 64 bits.  A weight's gradient sums some hundreds of fp32 products
+    through two layers: 1e-4 of its norm is 1000 u and more."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm().to(device)
+    dec = PagedGPT2Decoder(model, 4, 32, device, dtype=torch.float32, eos_token_id=3)
+    torch.manual_seed(0)
+    prompts, lengths = ragged_prompts(device)
+    out = dec.rollout(prompts, 12, lengths)
+    tokens, mask = out.get("tokens_response"), out.get("attention_mask_response")
+    width = int(lengths.max()) + 12
+    ids = torch.zeros(4, width, dtype=torch.long, device=device)
+    targets = torch.full((4, width), -100, device=device)
+    old = torch.zeros(4, width, device=device)
+    for b in range(4):
+        n = int(lengths[b])
+        ids[b, :n], ids[b, n:n + 12] = prompts[b, :n], tokens[b]
+        targets[b, n - 1:n + 11] = torch.where(mask[b], tokens[b], -100)
+        old[b, n - 1:n + 11] = out.get("log_probs")[b]
+    g = torch.Generator().manual_seed(1)
+    old = old + 0.2 * torch.randn(old.shape, generator=g).to(device)
+    td = TensorDict(
+        {"ids": ids, "targets": targets, "log_probs": old,
+         "advantage": torch.randn(4, 1, generator=g).to(device),
+         "ref_log_probs": old + 0.1 * torch.randn(old.shape, generator=g).to(device),
+         "attention_mask_response": targets != -100}, batch_size=[4])
+    loss = loss_cls(Actor(model), kl_to_ref_coeff=0.1, entropy_coeff=0.01)
+    vals = loss(td)
+    total = vals.get("loss_objective") + vals.get("loss_kl_to_ref") + vals.get("loss_entropy")
+    total.backward()
+    twin = make_lm().double()
+    twin.load_state_dict({k: v.double().cpu() for k, v in model.state_dict().items()})
+    td64 = TensorDict({k: (v.double() if v.is_floating_point() else v) for k, v in
+                       ((k, td.get(k).cpu()) for k in td.keys())}, batch_size=[4])
+    loss64 = loss_cls(Actor(twin, plain=True), kl_to_ref_coeff=0.1, entropy_coeff=0.01)
+    vals64 = loss64(td64)
+    total64 = vals64.get("loss_objective") + vals64.get("loss_kl_to_ref") + vals64.get("loss_entropy")
+    total64.backward()
+    for name in ("loss_objective", "loss_kl_to_ref", "loss_entropy", "kl_to_ref", "clip_fraction", "ESS"):
+        assert abs(float(vals.get(name).detach()) - float(vals64.get(name).detach())) < 1e-4, name
+    for (name, p), q in zip(model.named_parameters(), twin.parameters()):
+        off = (p.grad.cpu().double() - q.grad).norm()
+        assert off <= 1e-4 * q.grad.norm() + 1e-9, name
+
+
+class Given(TensorDictModuleBase):
+    """An actor whose log-probs are a leaf."""
+
+    def __init__(self, lp):
+        super().__init__()
+        self.lp = lp
+        self.in_keys, self.out_keys = [], ["log_probs"]
+
+    def forward(self, td):
+        td.set("log_probs", self.lp)
+        return td
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loss_cls", [GRPOLoss, DAPO, CISPOLoss])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("with_mask", [False, True])
+def test_grpo_family_on_the_gpu_equals_the_plain_form(loss_cls, reduction, with_mask):
+    g = torch.Generator().manual_seed(2)
+    old = -torch.rand(6, 33, generator=g) * 3
+    new = old + 0.3 * torch.randn(6, 33, generator=g)
+    data = dict(log_probs=old, advantage=torch.randn(6, generator=g),
+                ref_log_probs=old + 0.2 * torch.randn(6, 33, generator=g))
+    if with_mask:
+        data["attention_mask_response"] = (torch.rand(6, 33, generator=g) < 0.6).long()
+    else:
+        data["tokens_response"] = torch.zeros(6, 33, dtype=torch.long)
+
+    def run(device, dtype):
+        lp = new.to(device, dtype).requires_grad_()
+        loss = loss_cls(Given(lp), kl_to_ref_coeff=0.1, entropy_coeff=0.02, reduction=reduction)
+        vals = loss(TensorDict({k: v.to(device) if not v.is_floating_point() else v.to(device, dtype)
+                                for k, v in data.items()}, batch_size=[6]))
+        (grad,) = torch.autograd.grad(sum(vals.get(k) for k in vals.keys() if k.startswith("loss")), lp)
+        return {k: vals.get(k).detach().cpu().double() for k in vals.keys()}, grad.cpu().double(), vals
+
+    got, grad, vals = run("cuda", torch.float32)
+    want, dwant, _ = run("cpu", torch.float64)
+    assert got.keys() == want.keys()
+    n = 1 if reduction == "mean" else 198
+    for k in want:
+        # terms up to 30 in size, some 20 u each
+        assert abs(got[k] - want[k]) <= 20 * U * 30 * n, k
+    assert ((grad - dwant).abs() <= 64 * U * (dwant.abs() + 1.0)).all()
+    half, _, vals = run("cuda", torch.bfloat16)
+    assert vals.get("loss_objective").dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_grpo_subclass_keeps_its_own_gain():
+    class Own(GRPOLoss):
+        def _ratio_clip_gain(self, log_w, adv):
+            return log_w.exp() * adv * 0 + 7.0, log_w.exp()
+
+    lp = torch.zeros(2, 3, device="cuda", requires_grad=True)
+    td = TensorDict({"log_probs": torch.zeros(2, 3, device="cuda"),
+                     "advantage": torch.ones(2, 1, device="cuda")}, batch_size=[2])
+    assert float(Own(Given(lp))(td).get("loss_objective").detach()) == -7.0
+
+
+@pytest.mark.gpu
+def test_wrapper_log_probs_on_the_gpu():
+    from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
+
+    g = torch.Generator().manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = (torch.randn(2, 9, 503, generator=g) * 3).to(dtype).cuda()
+        tokens = torch.randint(0, 503, (2, 4), generator=g).cuda()
+        got = _log_probs_of(logits[:, 4:8], tokens)
+        want = logits[:, 4:8].double().log_softmax(-1).gather(-1, tokens[..., None]).squeeze(-1)
+        assert got.dtype == dtype
+        assert ((got.double() - want).abs() <= want.abs() * torch.finfo(dtype).eps + 1e-5).all()
+
+
+# --------------------------------------------------------------------------- #
+# streams, graphs, far offsets
+# --------------------------------------------------------------------------- #
+def decode_state(seed, batch=5, heads=8, kv_heads=2, dim=64, page=16, room=640):
+    """A cache long enough for the split attention; everything on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    columns = room // page
+    pages = batch * columns
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda").bfloat16()
+
+    return dict(
+        k_cache=normal(pages, kv_heads, page, dim), v_cache=normal(pages, kv_heads, page, dim),
+        page_table=torch.randperm(pages, generator=g, device="cuda").reshape(batch, columns).int(),
+        start=torch.randint(0, room - 1, (batch,), generator=g, device="cuda"),
+        q=normal(batch, 1, heads, dim), k=normal(batch, 1, kv_heads, dim), v=normal(batch, 1, kv_heads, dim),
+        rope=ops.rotary_table(room, dim, device="cuda"))
+
+
+def decode_step(s):
+    q = ops.paged_kv_append(s["k"], s["v"], s["k_cache"], s["v_cache"], s["page_table"], s["start"],
+                            q=s["q"], rope=s["rope"])
+    return ops.paged_attention_decode(
+        q[:, 0], s["k_cache"], s["v_cache"], s["page_table"], s["start"] + 1)
+
+
+def learn_step(logits, tokens, old, adv):
+    lp = ops.token_log_probs(logits, tokens)
+    out = ops.token_policy_loss(lp, old, adv, tokens != -100, old, kl_coeff=0.1)
+    (grad,) = torch.autograd.grad(out.loss_total, logits)
+    return out.loss_total.detach(), grad
+
+
+def learn_state(seed, rows=(3, 700), vocab=503):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    logits = torch.randn(*rows, vocab, generator=g, device="cuda").bfloat16().requires_grad_()
+    tokens = torch.randint(0, vocab, rows, generator=g, device="cuda")
+    tokens[:, -3:] = -100
+    old = -torch.rand(*rows, generator=g, device="cuda") * 8
+    return logits, tokens, old, torch.randn(rows[0], 1, generator=g, device="cuda")
+
+
+@pytest.mark.gpu
+def test_operators_on_side_streams():
+    """Two streams at once, each with its own step: every result is that of
+    the step alone."""
+    states, learn = [decode_state(i) for i in range(2)], [learn_state(i) for i in range(2)]
+    want = [decode_step(s).clone() for s in states]
+    dwant = [learn_step(*x) for x in learn]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append((decode_step(states[i]), learn_step(*learn[i])))
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(got[i][0], want[i])
+            assert torch.equal(got[i][1][0], dwant[i][0]) and torch.equal(got[i][1][1], dwant[i][1])
+
+
+@pytest.mark.gpu
+def test_operators_in_graphs():
+    """Two captured decode steps and a captured learning step, replayed in
+    turn with eager calls between, on changing inputs."""
+    states, x = [decode_state(i) for i in range(2)], learn_state(7, rows=(3, 8000))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in states:
+            decode_step(s)
+        learn_step(*x)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gc.collect()
+    graphs, outs = [], []
+    for s in states:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(decode_step(s))
+        graphs.append(graph)
+    learn_graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(learn_graph):
+        learned = learn_step(*x)
+    for r in range(4):
+        for i, s in enumerate(states):
+            fresh = decode_state(100 + 10 * r + i)
+            for name in ("q", "k", "v", "start", "page_table", "k_cache", "v_cache"):
+                s[name].copy_(fresh[name])
+        fresh = learn_state(200 + r, rows=(3, 8000))
+        with torch.no_grad():
+            for a, b in zip(x, fresh):
+                a.copy_(b)
+        for graph in graphs:
+            graph.replay()
+        learn_graph.replay()
+        other = decode_step(decode_state(5))  # allocates between the replays
+        torch.cuda.synchronize()
+        for s, o in zip(states, outs):
+            assert torch.equal(o, decode_step(s))
+        loss, grad = learn_step(*fresh)
+        assert torch.equal(learned[0], loss) and torch.equal(learned[1], grad)
+        del other, loss, grad
+
+
+@pytest.mark.gpu
+def test_cache_past_32_bits():
+    """Pages whose elements lie past 2**31 and, by position, at the end of a
+    long sequence."""
+    kv_heads, page, dim = 8, 64, 128
+    per = kv_heads * page * dim
+    pages = (1 << 31) // per + 40
+    k_cache = torch.empty(pages, kv_heads, page, dim, dtype=torch.bfloat16, device="cuda")
+    v_cache = torch.empty_like(k_cache)
+    table = torch.arange(pages - 20, pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    g = torch.Generator().manual_seed(0)
+    n = 20 * page
+    k, v = (torch.randn(1, n, kv_heads, dim, generator=g).bfloat16() for _ in range(2))
+    ops.paged_kv_append(k.cuda(), v.cuda(), k_cache, v_cache, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    for p in (0, 7, 19):
+        assert torch.equal(k_cache[pages - 1 - p].cpu(), k[0, p * page:(p + 1) * page].transpose(0, 1))
+        assert torch.equal(v_cache[pages - 1 - p].cpu(), v[0, p * page:(p + 1) * page].transpose(0, 1))
+    q = torch.randn(1, 16, dim, generator=g).bfloat16()
+    out = ops.paged_attention_decode(q.cuda(), k_cache, v_cache, table, torch.tensor([n], device="cuda")).cpu().double()
+    for h in range(16):
+        kk, vv = k[0, :, h // 2].double(), v[0, :, h // 2].double()
+        p = torch.softmax(kk @ q[0, h].double() / math.sqrt(dim), 0)
+        assert ((out[0, h] - p @ vv).abs() <= 2.0 ** -8 * (p @ vv).abs() + 2e-3 * (p @ vv.abs())).all()
+
+
+@pytest.mark.gpu
+def test_log_probs_past_32_bits():
+    rows, vocab = 42000, 51201
+    assert rows * vocab > 1 << 31
+    logits = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    tokens = torch.zeros(rows, dtype=torch.long, device="cuda")
+    logits[-1, 5] = 3.0
+    tokens[-1] = 5
+    logits.requires_grad_()
+    lp = ops.token_log_probs(logits, tokens)
+    (grad,) = torch.autograd.grad(lp, logits, torch.ones_like(lp))
+    s = math.exp(3.0) + vocab - 1
+    assert abs(float(lp[-1].detach()) - (3.0 - math.log(s))) < 1e-5
+    assert abs(float(lp[-2].detach()) + math.log(vocab)) < 1e-5
+    assert abs(float(grad[-1, 5]) - (1 - math.exp(3.0) / s)) < 2.0 ** -8
+    assert abs(float(grad[-1, 6]) + 1 / s) < 2.0 ** -8 / s
+    assert abs(float(grad[-2, -1]) + 1 / vocab) < 2.0 ** -8 / vocab
