@@ -207,16 +207,24 @@ int append_vec(const PagedAppendArgs& a, hipStream_t st) {
 // bound by the cache's bytes.  float32 caches use the fp32 matrix instruction on
 // tiles of 16 keys, with V's operand read directly.
 //
-// A wave owns whole tiles: while it computes one, the keys, values and page ids
-// of the next are on their way in its registers.  No barrier in the loop.
+// A wave owns whole tiles: while it computes one, the keys and values of the next
+// are on their way in its registers, and the page ids of the one after.  No barrier
+// in the loop.
 //
 // Work is split over the cache's length.  The tiles of all (sequence, key head)
 // items form one line, and worker w of W takes the tiles [w n / W, (w + 1) n / W)
 // of it, whatever items they belong to: ragged batches and single long sequences
-// fill the card alike, without the host knowing a length.  A worker's first and
-// last item may be shared with its neighbours; their parts (maximum, sum and
-// unnormalised output) go to its two workspace slots and a second launch joins
+// fill the card alike, without the host knowing a length.  A worker is a wave where
+// items are many, else a workgroup whose four waves take every fourth tile.  Its
+// first and last item may be shared with its neighbours; those parts (maximum, sum
+// and unnormalised output) go to its two workspace slots, and a second launch joins
 // them in order.  Sequences of length 0 count one empty tile and get zeros.
+//
+// Measured (one MI355X, where a large copy runs at 4.9 TB/s): 1 x 131072 keys, 32 +
+// 8 heads of 128 bf16, 98 us a call, 93 in the kernel (5.8 TB/s) and 5 in the join;
+// 48 sequences of 1 to 8192 keys 157 us (5.1 TB/s); 256 of 65 to 96 keys, 12 heads of
+// 64, 14 us (4.6 TB/s).  Bound by HBM; small calls by three dependent loads (length,
+// page id, key) and the launch.
 // ---------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -341,18 +349,40 @@ __device__ __forceinline__ long busy_workers(long workers, long total, int waves
   return workers < most ? workers : most;
 }
 
+// Orders a wave's own shared-memory writes before its reads of other lanes'
+// values, and the other way round.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // The dim that the next smaller DP takes: chunks below it are never past `dim`.
 template <int DP>
 constexpr int smaller_dim() {
   return DP <= 64 ? 0 : DP <= 96 ? 64 : DP <= 128 ? 96 : DP <= 192 ? 128 : 192;
 }
 
-// What one wave carries through its tiles of one item.
-template <typename T, int DP>
+// One (sequence, key head, head block) as a wave sees it.
+template <typename T>
+struct Item {
+  const int* table;
+  const T *k, *v;  // the key head's part of the caches
+  int len;
+};
+
+// What one wave carries through its tiles.  A tile goes through
+//
+//   pages     its page ids are asked for            (two tiles ahead)
+//   resolve   they become row addresses, fetch_k    (one tile ahead)
+//   scores    S = K Q^T; the key registers are free, fetch_k of the next tile
+//   weigh     the softmax's step, and the values leave their registers;
+//             fetch_v of the next tile
+//   gather    O += P V
+template <typename T, int DP, bool EXACT>  // EXACT: dim == DP
 struct Tiles;
 
 // 16-bit caches: tiles of 32 keys.
-template <typename T, int DP>
+template <typename T, int DP, bool EXACT>
 struct Tiles {
   using V8 = typename Matrix<T>::V8;
   static constexpr int KEYS = 32;
@@ -362,26 +392,60 @@ struct Tiles {
   static constexpr int PITCH = DP + 16;
   static constexpr int LDS_BYTES = KEYS * PITCH * 2;
   // whether chunks of column block j can lie past `dim`
-  static constexpr bool edge(int j) { return 32 * j + 32 > smaller_dim<DP>(); }
-  V8 q[J], k[2][J], v[2][J];
-  f32x4 acc[DP / 16];
+  static constexpr bool edge(int j) { return !EXACT && 32 * j + 32 > smaller_dim<DP>(); }
+  struct Query {
+    V8 x[J];
+  };
+  Query q;
+  V8 k[2][J], v[2][J], hi, lo;
+  f32x4 acc[DP / 16], s[2];
   float m, l;
+  int page[2];
+  unsigned ok[2], ok_next[2];  // bit i of [h]: key 16 h + i counts
+  long krow[2], vrow[2];
 
-  __device__ __forceinline__ void start(const T* qrow, bool live, int dim) {
+  static __device__ __forceinline__ Query query(const T* row, bool live, int dim) {
     const int chunk = (threadIdx.x & 63) >> 4;
+    Query q;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int d = (chunk + 4 * j) * 8;
-      q[j] = V8{};
-      if (live && d < dim) q[j] = *(const V8*)(qrow + d);
+      q.x[j] = V8{};
+      if (live && d < dim) q.x[j] = *(const V8*)(row + d);
     }
+    return q;
+  }
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
     l = 0.f;
   }
 
-  template <bool EXACT>
+  __device__ __forceinline__ void pages(const Item<T>& it, int shift, int tile) {
+    const int row = threadIdx.x & 15;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = tile * KEYS + 16 * h + row;
+      page[h] = key < it.len ? it.table[key >> shift] : -1;
+    }
+  }
+
+  // rows to read of a tile; keys that do not count read the cache's first row
+  __device__ __forceinline__ void resolve(const PagedCache& c, int tile) {
+    const int row = threadIdx.x & 15;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = tile * KEYS + 16 * h + row;
+      const bool fine = page[h] >= 0 && page[h] < c.pages;
+      const long slot = key & ((1 << c.page_shift) - 1);
+      krow[h] = fine ? page[h] * c.k_page + slot * c.k_slot : 0;
+      vrow[h] = fine ? page[h] * c.v_page + slot * c.v_slot : 0;
+      ok_next[h] = (unsigned)__ballot(fine) & 0xffffu;
+    }
+  }
+
   __device__ __forceinline__ void fetch(V8 (&x)[2][J], const T* base, const long (&row)[2], int dim) {
     const int chunk = (threadIdx.x & 63) >> 4;
 #pragma unroll
@@ -391,13 +455,14 @@ struct Tiles {
       for (int j = 0; j < J; ++j) {
         const int d = (chunk + 4 * j) * 8;
         // columns past dim: the row's first ones again, cleared before use
-        x[h][j] = *(const V8*)(p + (EXACT || !edge(j) || d < dim ? d : 0));
+        x[h][j] = *(const V8*)(p + (!edge(j) || d < dim ? d : 0));
       }
     }
   }
+  __device__ __forceinline__ void fetch_k(const Item<T>& it, int dim) { fetch(k, it.k, krow, dim); }
+  __device__ __forceinline__ void fetch_v(const Item<T>& it, int dim) { fetch(v, it.v, vrow, dim); }
 
-  template <bool EXACT>
-  __device__ __forceinline__ void scores(f32x4 (&s)[2], int dim) {
+  __device__ __forceinline__ void scores(int dim) {
     const int chunk = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -405,16 +470,15 @@ struct Tiles {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         V8 x = k[h][j];
-        if (!EXACT && edge(j) && (chunk + 4 * j) * 8 >= dim) x = V8{};
-        s[h] = Matrix<T>::mul(x, q[j], s[h]);
+        if (edge(j) && (chunk + 4 * j) * 8 >= dim) x = V8{};
+        s[h] = Matrix<T>::mul(x, q.x[j], s[h]);
       }
     }
   }
 
-  // `ok`: bit i of ok[h] says that key 16 h + i counts.
-  __device__ __forceinline__ void weigh(f32x4 (&s)[2], float scale, const unsigned (&ok)[2], bool full,
-                                        V8& hi, V8& lo) {
-    const int group = (threadIdx.x & 63) >> 4;
+  __device__ __forceinline__ void weigh(float scale, T* lds) {
+    const int lane = threadIdx.x & 63, row = lane & 15, group = lane >> 4;
+    const bool full = (ok[0] & ok[1]) == 0xffffu;
     float top = -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -444,23 +508,20 @@ struct Tiles {
         hi[4 * h + r] = (T)p;
         lo[4 * h + r] = (T)(p - (float)hi[4 * h + r]);
       }
-  }
-
-  __device__ __forceinline__ void stage(T* lds, const unsigned (&ok)[2], bool full) {
-    const int lane = threadIdx.x & 63, row = lane & 15, chunk = lane >> 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool clear = !full && !((ok[h] >> row) & 1);
+      const bool gone = !full && !((ok[h] >> row) & 1);
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        *(V8*)(lds + (16 * h + row) * PITCH + (chunk + 4 * j) * 8) = clear ? V8{} : v[h][j];
+        *(V8*)(lds + (16 * h + row) * PITCH + (group + 4 * j) * 8) = gone ? V8{} : v[h][j];
     }
   }
 
-  __device__ __forceinline__ void gather(const T* lds, V8 hi, V8 lo) {
+  __device__ __forceinline__ void gather(const T* lds) {
     const int lane = threadIdx.x & 63, i = lane & 15, group = lane >> 4;
     const T* p = lds + (4 * group + i / 4) * PITCH + (i % 4) * 4;
     typedef __attribute__((address_space(3))) s16x4* Shared;
+    wave_sync();
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
       union {
@@ -472,194 +533,215 @@ struct Tiles {
       acc[d] = Matrix<T>::mul(x.all, hi, acc[d]);
       acc[d] = Matrix<T>::mul(x.all, lo, acc[d]);
     }
+    wave_sync();
   }
-};
 
-// Orders a wave's own shared-memory writes before its reads of other lanes'
-// values, and the other way round.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
-template <typename T, int DP, bool EXACT>
-__device__ __forceinline__ void run_tiles(Tiles<T, DP>& w, const PagedAttendArgs& a, long b, int kv,
-                                          int len, int t, int end, int step, T* lds) {
-  constexpr int KEYS = Tiles<T, DP>::KEYS;
-  const int row = threadIdx.x & 15;
-  const int* table = a.cache.table + b * a.cache.table_stride;
-  const T* kbase = (const T*)a.cache.k + kv * a.cache.k_head;
-  const T* vbase = (const T*)a.cache.v + kv * a.cache.v_head;
-  const int slot_mask = (1 << a.cache.page_shift) - 1;
-  int page[2];
-  unsigned ok[2], ok_next[2];
-  long krow[2], vrow[2];
-  auto pages = [&](int tile) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = tile * KEYS + 16 * h + row;
-      page[h] = key < len ? table[key >> a.cache.page_shift] : -1;
-    }
-  };
-  // rows to read of a tile; keys that do not count read the cache's first row
-  auto resolve = [&](int tile, unsigned (&good)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = tile * KEYS + 16 * h + row;
-      const bool fine = page[h] >= 0 && page[h] < a.cache.pages;
-      const long slot = key & slot_mask;
-      krow[h] = fine ? page[h] * a.cache.k_page + slot * a.cache.k_slot : 0;
-      vrow[h] = fine ? page[h] * a.cache.v_page + slot * a.cache.v_slot : 0;
-      good[h] = (unsigned)__ballot(fine) & 0xffffu;
-    }
-  };
-  if (t >= end) return;
-  pages(t);
-  resolve(t, ok);
-  if (t + step < end) pages(t + step);
-  w.template fetch<EXACT>(w.k, kbase, krow, a.dim);
-  w.template fetch<EXACT>(w.v, vbase, vrow, a.dim);
-  for (; t < end; t += step) {
-    const bool more = t + step < end;
-    if (more) {
-      resolve(t + step, ok_next);
-      if (t + 2 * step < end) pages(t + 2 * step);  // ahead of the loads that follow
-    }
-    f32x4 s[2];
-    typename Tiles<T, DP>::V8 hi, lo;
-    w.template scores<EXACT>(s, a.dim);
-    if (more) w.template fetch<EXACT>(w.k, kbase, krow, a.dim);
-    const bool full = (ok[0] & ok[1]) == 0xffffu;
-    w.weigh(s, a.scale, ok, full, hi, lo);
-    w.stage(lds, ok, full);
-    if (more) w.template fetch<EXACT>(w.v, vbase, vrow, a.dim);
-    wave_sync();
-    w.gather(lds, hi, lo);
-    wave_sync();
+  __device__ __forceinline__ void turn_over() {
     ok[0] = ok_next[0];
     ok[1] = ok_next[1];
   }
-}
+};
 
-// float32 caches: tiles of 16 keys, the fp32 matrix instruction.
-template <int DP>
-struct Tiles<float, DP> {
+// float32 caches: tiles of 16 keys, the fp32 matrix instruction, V's operand
+// straight from the cache.
+template <int DP, bool EXACT>
+struct Tiles<float, DP, EXACT> {
   static constexpr int KEYS = 16;
   static constexpr int J = DP / 16;
   static constexpr int LDS_BYTES = 16 * (DP + 4) * 4;  // the join's only
-  static constexpr bool edge(int j) { return 16 * j + 16 > smaller_dim<DP>(); }
-  f32x4 q[J], k[J], v[J], acc[J];  // v[d][r]: dim 16 d + l % 16 of key 4 (l / 16) + r
+  static constexpr bool edge(int j) { return !EXACT && 16 * j + 16 > smaller_dim<DP>(); }
+  struct Query {
+    f32x4 x[J];
+  };
+  Query q;
+  f32x4 k[J], v[J], acc[J], s;  // v[d][r]: dim 16 d + l % 16 of key 4 (l / 16) + r
   float m, l;
+  int page;
+  unsigned ok, ok_next;
+  long krow, vrow;
 
-  __device__ __forceinline__ void start(const float* qrow, bool live, int dim) {
+  static __device__ __forceinline__ Query query(const float* row, bool live, int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
+    Query q;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int d = (chunk + 4 * j) * 4;
+      q.x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (live && d < dim) q.x[j] = *(const f32x4*)(row + d);
+    }
+    return q;
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < J; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  __device__ __forceinline__ void pages(const Item<float>& it, int shift, int tile) {
+    const int key = tile * KEYS + (threadIdx.x & 15);
+    page = key < it.len ? it.table[key >> shift] : -1;
+  }
+
+  __device__ __forceinline__ void resolve(const PagedCache& c, int tile) {
+    const int key = tile * KEYS + (threadIdx.x & 15);
+    const bool fine = page >= 0 && page < c.pages;
+    const long slot = key & ((1 << c.page_shift) - 1);
+    krow = fine ? page * c.k_page + slot * c.k_slot : 0;
+    vrow = fine ? page * c.v_page + slot * c.v_slot : 0;
+    ok_next = (unsigned)__ballot(fine) & 0xffffu;
+  }
+
+  __device__ __forceinline__ void fetch_k(const Item<float>& it, int dim) {
     const int chunk = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int d = (chunk + 4 * j) * 4;
-      q[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (live && d < dim) q[j] = *(const f32x4*)(qrow + d);
-      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      k[j] = *(const f32x4*)(it.k + krow + (!edge(j) || d < dim ? d : 0));
     }
-    m = -INFINITY;
-    l = 0.f;
   }
-};
 
-template <int DP, bool EXACT>
-__device__ __forceinline__ void run_tiles_f32(Tiles<float, DP>& w, const PagedAttendArgs& a, long b,
-                                              int kv, int len, int t, int end, int step) {
-  constexpr int J = DP / 16;
-  const int lane = threadIdx.x & 63, row = lane & 15, chunk = lane >> 4;
-  const int* table = a.cache.table + b * a.cache.table_stride;
-  const float* kbase = (const float*)a.cache.k + kv * a.cache.k_head;
-  const float* vbase = (const float*)a.cache.v + kv * a.cache.v_head;
-  const int slot_mask = (1 << a.cache.page_shift) - 1;
-  int page = -1;
-  unsigned ok = 0, ok_next = 0;
-  long krow = 0, vrow = 0;
-  auto pages = [&](int tile) {
-    const int key = tile * 16 + row;
-    page = key < len ? table[key >> a.cache.page_shift] : -1;
-  };
-  auto resolve = [&](int tile, unsigned& good) {
-    const int key = tile * 16 + row;
-    const bool fine = page >= 0 && page < a.cache.pages;
-    const long slot = key & slot_mask;
-    krow = fine ? page * a.cache.k_page + slot * a.cache.k_slot : 0;
-    vrow = fine ? page * a.cache.v_page + slot * a.cache.v_slot : 0;
-    good = (unsigned)__ballot(fine) & 0xffffu;
-  };
-  auto fetch_k = [&]() {
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int d = (chunk + 4 * j) * 4;
-      w.k[j] = *(const f32x4*)(kbase + krow + (EXACT || !w.edge(j) || d < a.dim ? d : 0));
-    }
-  };
-  auto fetch_v = [&]() {
+  __device__ __forceinline__ void fetch_v(const Item<float>& it, int dim) {
+    const int lane = threadIdx.x & 63, row = lane & 15, chunk = lane >> 4;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float* p = vbase + __shfl(vrow, 4 * chunk + r, 64);
+      const float* p = it.v + __shfl(vrow, 4 * chunk + r, 64);
 #pragma unroll
       for (int d = 0; d < J; ++d) {
         const int col = 16 * d + row;
-        w.v[d][r] = p[EXACT || !w.edge(d) || col < a.dim ? col : 0];
+        v[d][r] = p[!edge(d) || col < dim ? col : 0];
       }
     }
-  };
-  if (t >= end) return;
-  pages(t);
-  resolve(t, ok);
-  if (t + step < end) pages(t + step);
-  fetch_k();
-  fetch_v();
-  for (; t < end; t += step) {
-    const bool more = t + step < end;
-    if (more) {
-      resolve(t + step, ok_next);
-      if (t + 2 * step < end) pages(t + 2 * step);
-    }
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  }
+
+  __device__ __forceinline__ void scores(int dim) {
+    const int chunk = (threadIdx.x & 63) >> 4;
+    s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      f32x4 x = w.k[j];
-      if (!EXACT && w.edge(j) && (chunk + 4 * j) * 4 >= a.dim) x = f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 x = k[j];
+      if (edge(j) && (chunk + 4 * j) * 4 >= dim) x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w.q[j][i], s, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], q.x[j][i], s, 0, 0, 0);
     }
-    if (more) fetch_k();
+  }
+
+  __device__ __forceinline__ void weigh(float scale, float*) {
+    const int chunk = (threadIdx.x & 63) >> 4;
     const bool full = ok == 0xffffu;
     float top = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      s[r] *= a.scale;
+      s[r] *= scale;
       if (!full && !((ok >> (4 * chunk + r)) & 1)) s[r] = -INFINITY;
       top = fmaxf(top, s[r]);
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > w.m)) {
-      const float next = fmaxf(w.m, top);
-      const float keep = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - next);
-      w.m = next;
-      w.l *= keep;
+    if (__any(top > m)) {
+      const float next = fmaxf(m, top);
+      const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= keep;
 #pragma unroll
-      for (int i = 0; i < J; ++i) w.acc[i] *= keep;
+      for (int i = 0; i < J; ++i) acc[i] *= keep;
     }
-    const float off = w.m == -INFINITY ? 0.f : w.m;
+    const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float p = __builtin_amdgcn_exp2f(s[r] - off);
-      w.l += p;
+      l += p;
       const bool gone = !full && !((ok >> (4 * chunk + r)) & 1);
 #pragma unroll
       for (int d = 0; d < J; ++d)
-        w.acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(gone ? 0.f : w.v[d][r], p, w.acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(gone ? 0.f : v[d][r], p, acc[d], 0, 0, 0);
     }
-    if (more) fetch_v();
-    ok = ok_next;
   }
+
+  __device__ __forceinline__ void gather(const float*) {}
+  __device__ __forceinline__ void turn_over() { ok = ok_next; }
+};
+
+template <typename T>
+__device__ __forceinline__ Item<T> item_of(const PagedAttendArgs& a, const AttendPlan& plan, long b,
+                                           int item) {
+  const int kv = item / plan.blocks;
+  const long room = (long)a.cache.table_cols << a.cache.page_shift;
+  const long len = whole(a.lengths, a.lengths_i64, b);
+  return {a.cache.table + b * a.cache.table_stride, (const T*)a.cache.k + kv * a.cache.k_head,
+          (const T*)a.cache.v + kv * a.cache.v_head, (int)(len < room ? len : room)};
+}
+
+// The first query head of an item and how many it has.
+struct Heads {
+  int first, count;
+};
+
+__device__ __forceinline__ Heads heads_of(const PagedAttendArgs& a, const AttendPlan& plan, int item) {
+  const int group = a.heads / a.kv_heads, kv = item / plan.blocks;
+  const int first = kv * group + 16 * (item % plan.blocks);
+  return {first, min(16, (kv + 1) * group - first)};
+}
+
+template <typename W, typename T>
+__device__ __forceinline__ typename W::Query query_of(const PagedAttendArgs& a, long b, Heads h) {
+  const int mine = threadIdx.x & 15;
+  const bool live = mine < h.count;
+  return W::query((const T*)a.q + b * a.q_batch + (h.first + (live ? mine : 0)) * a.q_head, live, a.dim);
+}
+
+// A place on the line of tiles.
+struct Cursor {
+  long b;
+  int item, at, tiles;  // at < tiles of the item
+};
+
+// The range of the line that worker `me` takes, and its note for the join.
+struct Range {
+  Cursor from;
+  int count;
+  SharedItem note;
+};
+
+__device__ __forceinline__ Range range_of(const PagedAttendArgs& a, const AttendPlan& plan, int keys,
+                                          int waves) {
+  const long me = blockIdx.x;
+  const int per = a.kv_heads * plan.blocks;
+  Range x;
+  x.note = {0, 0, 0, 0, 0};
+  if (plan.workers == 0) {
+    const long b = (unsigned)me / (unsigned)per;
+    const int tiles = tiles_of(a, b, keys);
+    x.from = {b, (int)(me - b * per), 0, tiles};
+    x.count = tiles;
+    return x;
+  }
+  const Line line = line_of(a, per, keys);
+  const long busy = busy_workers(plan.workers, line.total, waves);
+  x.count = 0;
+  x.from = {0, 0, 0, 1};
+  if (me < busy) {
+    const long lo = share(me, line.total, busy), hi = share(me + 1, line.total, busy);
+    const Spot s = spot_of(a, per, keys, line, lo);
+    const int item = (int)share(lo - s.first, 1, s.tiles);
+    const int at = (int)(lo - s.first - (long)item * s.tiles);
+    x.from = {s.b, item, at, s.tiles};
+    x.count = (int)(hi - lo);
+    if (at > 0) {
+      // the first border strictly inside an item answers for its join
+      const long from = lo - at, before = share(me - 1, line.total, busy);
+      if (before <= from) {
+        // the worker of the item's last tile is the last whose range begins at or
+        // before it: ceil(end * busy / total) - 1
+        const long end = from + s.tiles, last = share(end, busy, line.total);
+        const int w1 = (int)(last * line.total == end * busy ? last - 1 : last);
+        x.note = {s.b, item, (int)me - 1, w1 - (int)me + 2, 2 * ((int)me - 1) + (before == from ? 0 : 1)};
+      }
+    }
+  }
+  if (threadIdx.x == 0) plan.notes[me] = x.note;
+  return x;
 }
 
 // Waves to a SIMD that the registers are held to.
@@ -667,10 +749,116 @@ constexpr int resident_waves(int dim, int size) {
   return dim <= 96 ? 3 : dim <= 128 || (size == 2 && dim <= 192) ? 2 : 1;
 }
 
-template <typename T, int DP, bool EXACT, int NW>
-__global__ __launch_bounds__(64 * NW, resident_waves(DP, sizeof(T))) void paged_attend_k(
+// Many items: a wave is a worker by itself.  Its tiles run on over the borders of
+// items, the next item's first keys on their way while the last one ends.
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_attend_wave_k(
     const PagedAttendArgs a, const AttendPlan plan) {
-  using W = Tiles<T, DP>;
+  using W = Tiles<T, DP, EXACT>;
+  __shared__ __attribute__((aligned(16))) char lds[sizeof(T) == 2 ? W::LDS_BYTES : 16];
+  const int lane = threadIdx.x;
+  const int per = a.kv_heads * plan.blocks;
+  const int group = a.heads / a.kv_heads;
+  const int rows = group < 16 ? group : 16;
+  const int shift = a.cache.page_shift;
+  const Range range = range_of(a, plan, W::KEYS, 1);
+  if (range.count == 0) return;
+
+  auto after = [&](Cursor c) {
+    if (++c.at == c.tiles) {
+      c.at = 0;
+      if (++c.item == per) {
+        c.item = 0;
+        if (c.b + 1 < a.batch) c.tiles = tiles_of(a, ++c.b, W::KEYS);
+      }
+    }
+    return c;
+  };
+  Cursor now = range.from, next = after(now), far = after(next);
+  Item<T> it = item_of<T>(a, plan, now.b, now.item);
+  Heads heads = heads_of(a, plan, now.item);
+  W w;
+  typename W::Query q;
+  w.q = query_of<W, T>(a, now.b, heads);
+  w.clear();
+  w.pages(it, shift, now.at);
+  w.resolve(a.cache, now.at);
+  w.turn_over();
+  const Item<T> first = it;
+  if (range.count > 1) {
+    it = item_of<T>(a, plan, next.b, next.item);
+    w.pages(it, shift, next.at);
+  }
+  w.fetch_k(first, a.dim);
+  w.fetch_v(first, a.dim);
+  int begin = now.at;  // where this worker's part of the item begins
+  long slot = 2 * (long)blockIdx.x;
+  for (int i = 0; i < range.count; ++i) {
+    const bool more = i + 1 < range.count;
+    const bool last = !more || next.at == 0;  // of this item here
+    const Item<T> ahead = it;                  // of `next`
+    if (more) {
+      w.resolve(a.cache, next.at);
+      if (i + 2 < range.count) {
+        it = item_of<T>(a, plan, far.b, far.item);
+        w.pages(it, shift, far.at);  // ahead of the loads that follow
+      }
+      if (last) q = query_of<W, T>(a, next.b, heads_of(a, plan, next.item));
+    }
+    w.scores(a.dim);
+    if (more) w.fetch_k(ahead, a.dim);
+    w.weigh(a.scale, (T*)lds);
+    if (more) w.fetch_v(ahead, a.dim);
+    w.gather((const T*)lds);
+    if (last) {
+      float sum = w.l;
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      const int g = lane & 15, d0 = 4 * (lane >> 4);
+      if (g < heads.count) {
+        if (begin > 0 || now.at + 1 < now.tiles) {
+          float* p = plan.part + (slot * rows + g) * a.dim + d0;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d)
+            if (16 * d + d0 < a.dim) *(f32x4*)(p + 16 * d) = w.acc[d];
+          if (lane < 16) {
+            plan.part_ms[(slot * rows + g) * 2] = w.m;
+            plan.part_ms[(slot * rows + g) * 2 + 1] = sum;
+          }
+        } else {
+          T* p = (T*)a.out + (now.b * a.heads + heads.first + g) * a.dim + d0;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d)
+            if (16 * d + d0 < a.dim) {
+              Chunk<T, 4> o;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o.x[r] = (T)(sum == 0.f ? 0.f : w.acc[d][r] / sum);
+              *(Chunk<T, 4>*)(p + 16 * d) = o;
+            }
+        }
+      }
+      if (more) {
+        heads = heads_of(a, plan, next.item);
+        w.q = q;
+        w.clear();
+        begin = 0;
+        slot = 2 * (long)blockIdx.x + 1;
+      }
+    }
+    w.turn_over();
+    now = next;
+    next = far;
+    if (i + 3 < range.count) far = after(far);
+  }
+}
+
+// Few items: the four waves of a workgroup share a worker's tiles and join what
+// they have at the end of each item.
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(256, resident_waves(DP, sizeof(T))) void paged_attend_group_k(
+    const PagedAttendArgs a, const AttendPlan plan) {
+  using W = Tiles<T, DP, EXACT>;
+  constexpr int NW = 4;
   constexpr int OUT = DP + 4;  // pitch of a head's output in shared memory
   static_assert(16 * OUT * 4 <= W::LDS_BYTES, "the join reuses the staging rows");
   __shared__ __attribute__((aligned(16))) char lds[NW][W::LDS_BYTES];
@@ -679,73 +867,54 @@ __global__ __launch_bounds__(64 * NW, resident_waves(DP, sizeof(T))) void paged_
   const int group = a.heads / a.kv_heads;
   const int per = a.kv_heads * plan.blocks;  // items of a sequence
   const int rows = group < 16 ? group : 16;
-  const long room = (long)a.cache.table_cols << a.cache.page_shift;
-
-  long b;
-  int item, tiles, at, left;  // `left`: tiles still to do, over items
-  SharedItem note = {0, 0, 0, 0, 0};
-  if (plan.workers == 0) {
-    b = blockIdx.x / per;
-    item = (int)(blockIdx.x % per);
-    tiles = left = tiles_of(a, b, W::KEYS);
-    at = 0;
-  } else {
-    const Line line = line_of(a, per, W::KEYS);
-    const long busy = busy_workers(plan.workers, line.total, NW);
-    if (blockIdx.x >= busy) {
-      if (threadIdx.x == 0) plan.notes[blockIdx.x] = note;
-      return;
-    }
-    const long lo = share(blockIdx.x, line.total, busy), hi = share(blockIdx.x + 1, line.total, busy);
-    const Spot s = spot_of(a, per, W::KEYS, line, lo);
-    b = s.b;
-    tiles = s.tiles;
-    item = (int)share(lo - s.first, 1, tiles);
-    at = (int)(lo - s.first - (long)item * tiles);
-    left = (int)(hi - lo);
-    if (at > 0) {
-      // the first border strictly inside an item answers for its join
-      const long from = lo - at, before = share(blockIdx.x - 1, line.total, busy);
-      if (before <= from) {
-        // the worker of the item's last tile is the last whose range begins at or
-        // before it: ceil(end * busy / total) - 1
-        const long end = from + tiles, last = share(end, busy, line.total);
-        const int w1 = (int)(last * line.total == end * busy ? last - 1 : last);
-        note = {b, item, (int)blockIdx.x - 1, w1 - (int)blockIdx.x + 2,
-                2 * ((int)blockIdx.x - 1) + (before == from ? 0 : 1)};
-      }
-    }
-    if (threadIdx.x == 0) plan.notes[blockIdx.x] = note;
-  }
+  const int shift = a.cache.page_shift;
+  const Range range = range_of(a, plan, W::KEYS, NW);
+  Cursor now = range.from;
+  int left = range.count;  // tiles still to do, over items
   bool first = true;
   while (left > 0) {
-    const int end = left < tiles - at ? at + left : tiles;
-    long len = whole(a.lengths, a.lengths_i64, b);
-    len = len < room ? len : room;
-    const int kv = item / plan.blocks;
-    const int head0 = kv * group + 16 * (item % plan.blocks);  // the first of this block
-    const int heads = min(16, (kv + 1) * group - head0);
+    const int end = left < now.tiles - now.at ? now.at + left : now.tiles;
+    const Item<T> it = item_of<T>(a, plan, now.b, now.item);
+    const Heads heads = heads_of(a, plan, now.item);
     W w;
-    const bool live = (lane & 15) < heads;
-    w.start((const T*)a.q + b * a.q_batch + (head0 + (live ? lane & 15 : 0)) * a.q_head, live, a.dim);
-    if constexpr (sizeof(T) == 4)
-      run_tiles_f32<DP, EXACT>(w, a, b, kv, (int)len, at + wave, end, NW);
-    else
-      run_tiles<T, DP, EXACT>(w, a, b, kv, (int)len, at + wave, end, NW, (T*)lds[wave]);
+    w.q = query_of<W, T>(a, now.b, heads);
+    w.clear();
+    T* mine = (T*)lds[wave];
+    int t = now.at + wave;
+    if (t < end) {
+      w.pages(it, shift, t);
+      w.resolve(a.cache, t);
+      w.turn_over();
+      if (t + NW < end) w.pages(it, shift, t + NW);
+      w.fetch_k(it, a.dim);
+      w.fetch_v(it, a.dim);
+      for (; t < end; t += NW) {
+        const bool more = t + NW < end;
+        if (more) {
+          w.resolve(a.cache, t + NW);
+          if (t + 2 * NW < end) w.pages(it, shift, t + 2 * NW);  // ahead of the loads that follow
+        }
+        w.scores(a.dim);
+        if (more) w.fetch_k(it, a.dim);
+        w.weigh(a.scale, mine);
+        if (more) w.fetch_v(it, a.dim);
+        w.gather(mine);
+        w.turn_over();
+      }
+    }
     w.l += __shfl_xor(w.l, 16, 64);
     w.l += __shfl_xor(w.l, 32, 64);
-    wave_sync();
-    float* mine = (float*)lds[wave] + (lane & 15) * OUT + 4 * (lane >> 4);
+    float* put = (float*)lds[wave] + (lane & 15) * OUT + 4 * (lane >> 4);
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) *(f32x4*)(mine + 16 * d) = w.acc[d];
+    for (int d = 0; d < DP / 16; ++d) *(f32x4*)(put + 16 * d) = w.acc[d];
     if (lane < 16) {
       sm[wave][lane] = w.m;
       sl[wave][lane] = w.l;
     }
     __syncthreads();
-    const bool shared = at > 0 || end < tiles;
+    const bool shared = now.at > 0 || end < now.tiles;
     const long slot = 2 * (long)blockIdx.x + (first ? 0 : 1);
-    for (int i = threadIdx.x; i < heads * a.dim; i += 64 * NW) {
+    for (int i = threadIdx.x; i < heads.count * a.dim; i += 64 * NW) {
       const int g = i / a.dim, d = i - g * a.dim;
       float top = sm[0][g];
 #pragma unroll
@@ -764,18 +933,17 @@ __global__ __launch_bounds__(64 * NW, resident_waves(DP, sizeof(T))) void paged_
           plan.part_ms[(slot * rows + g) * 2 + 1] = sum;
         }
       } else {
-        ((T*)a.out)[(b * a.heads + head0 + g) * a.dim + d] = (T)(sum == 0.f ? 0.f : out / sum);
+        ((T*)a.out)[(now.b * a.heads + heads.first + g) * a.dim + d] = (T)(sum == 0.f ? 0.f : out / sum);
       }
     }
     first = false;
-    left -= end - at;
-    at = 0;
+    left -= end - now.at;
+    now.at = 0;
     if (left > 0) {
       __syncthreads();  // the rows above are staged into again
-      if (++item == per) {
-        item = 0;
-        ++b;
-        tiles = tiles_of(a, b, W::KEYS);
+      if (++now.item == per) {
+        now.item = 0;
+        now.tiles = tiles_of(a, ++now.b, W::KEYS);
       }
     }
   }
@@ -853,35 +1021,92 @@ __global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs
   for (int r = 0; r < 4; ++r) dst[r] = (T)(sum == 0.f ? 0.f : out[r] / sum);
 }
 
-template <typename T, int DP, bool EXACT>
-int attend_launch(const PagedAttendArgs& a, hipStream_t st) {
-  const AttendPlan plan{a.workers, a.head_blocks, (SharedItem*)a.notes, a.part, a.part_ms};
-  const int per = a.kv_heads * a.head_blocks;
-  const long items = a.batch * per;
-  const dim3 blocks((unsigned)(a.workers ? a.workers : items));
-  if (a.waves == 1)
-    hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 1>), blocks, dim3(64), 0, st, a, plan);
-  else
-    hipLaunchKernelGGL((paged_attend_k<T, DP, EXACT, 4>), blocks, dim3(256), 0, st, a, plan);
-  if (a.workers < 2) return (int)hipGetLastError();
+// The same where single waves are the workers: items are many and their parts
+// few, so a thread takes 4 values of an item and all its parts.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_attend_join_few_k(const PagedAttendArgs a,
+                                                               const AttendPlan plan) {
   const int group = a.heads / a.kv_heads;
-  const dim3 grid((unsigned)a.workers, (unsigned)(((group < 16 ? group : 16) * a.dim + 127) / 128));
-  hipLaunchKernelGGL((paged_attend_join_k<T>), grid, dim3(256), 0, st, a, plan);
-  return (int)hipGetLastError();
+  const int rows = group < 16 ? group : 16;
+  const unsigned quads = a.dim / 4, all = rows * quads;
+  const unsigned id = blockIdx.x * 256 + threadIdx.x;
+  if (id / all >= (unsigned)plan.workers) return;
+  const SharedItem note = plan.notes[id / all];
+  const int g = (int)(id % all / quads), quad = (int)(id % quads);
+  const Heads heads = heads_of(a, plan, note.item);
+  if (note.parts == 0 || g >= heads.count) return;
+  float top = -INFINITY, sum = 0.f;
+  f32x4 out = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 4;
+  for (int i0 = 0; i0 < note.parts; i0 += N) {
+    float m[N], l[N];
+    f32x4 x[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = min(i0 + u, note.parts - 1);
+      const long row = (i == 0 ? note.slot : 2 * (long)(note.worker + i)) * rows + g;
+      m[u] = plan.part_ms[2 * row];
+      l[u] = plan.part_ms[2 * row + 1];
+      x[u] = *(const f32x4*)(plan.part + row * a.dim + 4 * quad);
+    }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < N; ++u) next = fmaxf(next, m[u]);
+    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    top = next;
+    sum *= keep;
+    out *= keep;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (i0 + u >= note.parts) continue;
+      const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+      sum += f * l[u];
+      out += f * x[u];
+    }
+  }
+  T* dst = (T*)a.out + (note.b * a.heads + heads.first + g) * a.dim + 4 * quad;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) dst[r] = (T)(sum == 0.f ? 0.f : out[r] / sum);
 }
 
-template <typename T, int DP>
-int attend_dim(const PagedAttendArgs& a, hipStream_t st) {
-  return a.dim == DP ? attend_launch<T, DP, true>(a, st) : attend_launch<T, DP, false>(a, st);
+template <typename T, int DP, bool EXACT>
+void attend_kernel(const PagedAttendArgs& a, const AttendPlan& plan, hipStream_t st) {
+  const dim3 blocks((unsigned)(a.workers ? a.workers : a.batch * a.kv_heads * a.head_blocks));
+  if (a.waves == 1)
+    hipLaunchKernelGGL((paged_attend_wave_k<T, DP, EXACT>), blocks, dim3(64), 0, st, a, plan);
+  else
+    hipLaunchKernelGGL((paged_attend_group_k<T, DP, EXACT>), blocks, dim3(256), 0, st, a, plan);
 }
 
 template <typename T>
 int attend_any(const PagedAttendArgs& a, hipStream_t st) {
-  if (a.dim <= 64) return attend_dim<T, 64>(a, st);
-  if (a.dim <= 96) return attend_dim<T, 96>(a, st);
-  if (a.dim <= 128) return attend_dim<T, 128>(a, st);
-  if (a.dim <= 192) return attend_dim<T, 192>(a, st);
-  return attend_dim<T, 256>(a, st);
+  const AttendPlan plan{a.workers, a.head_blocks, (SharedItem*)a.notes, a.part, a.part_ms};
+  if (a.dim < 64)
+    attend_kernel<T, 64, false>(a, plan, st);
+  else if (a.dim == 64)
+    attend_kernel<T, 64, true>(a, plan, st);
+  else if (a.dim <= 96)
+    attend_kernel<T, 96, false>(a, plan, st);
+  else if (a.dim < 128)
+    attend_kernel<T, 128, false>(a, plan, st);
+  else if (a.dim == 128)
+    attend_kernel<T, 128, true>(a, plan, st);
+  else if (a.dim <= 192)
+    attend_kernel<T, 192, false>(a, plan, st);
+  else if (a.dim < 256)
+    attend_kernel<T, 256, false>(a, plan, st);
+  else
+    attend_kernel<T, 256, true>(a, plan, st);
+  if (a.workers < 2) return (int)hipGetLastError();
+  const int group = a.heads / a.kv_heads;
+  const long quads = (long)(group < 16 ? group : 16) * (a.dim / 4);
+  if (a.waves == 1)
+    hipLaunchKernelGGL((paged_attend_join_few_k<T>), dim3((unsigned)((a.workers * quads + 255) / 256)),
+                       dim3(256), 0, st, a, plan);
+  else
+    hipLaunchKernelGGL((paged_attend_join_k<T>), dim3((unsigned)a.workers, (unsigned)((quads + 31) / 32)),
+                       dim3(256), 0, st, a, plan);
+  return (int)hipGetLastError();
 }
 
 }  // namespace
@@ -889,20 +1114,25 @@ int attend_any(const PagedAttendArgs& a, hipStream_t st) {
 extern "C" long paged_attend_note_bytes(void) { return (long)sizeof(SharedItem); }
 
 // How a call is split, by what the host knows: the table's columns bound every
-// length.  Measured in us, 16-bit caches, the other choice in brackets:
+// length.  Measured in us with the other choice in brackets (bf16, keys by page
+// tables of 64):
 //
-// - Short tables take one workgroup per item and no join, of one wave where
-//   there are items to fill the card: 2048 items of 16 tiles 99 [split: 108],
-//   3072 of 16 74 [80]; 4096 of 4 tiles 57 [four waves: 74].  Longer ones are
-//   split, for ragged batches: what a direct call wins at equal lengths (768
-//   items of 32 tiles 39 [43]) it loses on the longest item of others.
-// - A split call gives a CU one workgroup of 4 waves for dims above 96, where
-//   their tiles on the way (128 dim bytes to a wave) cover the latency, and two
-//   below: 1 x 131072 keys, 8 heads of 128: 101 [104 with two, 113 with three];
-//   2 heads of 256, 65536 keys: 40 [54]; 48 x 4096, 12 heads of 64: 113 [120
-//   with one].  More workers only add prologues and parts to join.
+// - Short tables take one worker per item and no join: 2048 items of 16 tiles,
+//   dim 128, 100 [split: 106]; 3072 of 16, dim 64, 74 [83]; 4096 of 4 57 [65].
+// - From 256 items on a worker is one wave, below a workgroup of four: ragged
+//   lengths of 1 to 1024, 768 items of dim 64, 28 [51]; 512 of dim 128 39 [64]; 1
+//   to 8192, 384 of dim 128, 160 [171]; but 16 items of 1 to 30000 38 [45], 8 of
+//   131072 101 [114].  Equal lengths gain less or lose: 384 items of 4096 153 [144].
+// - Workers are as many as fill the card once, no more: each has a start of its
+//   own, and shares items that must be joined.  Single waves two to a SIMD: 512
+//   items of 1 to 1024, dim 128, 41 [49 with one, 44 with three].  Workgroups one
+//   to a CU for dims above 96, whose tiles on the way (128 dim bytes to a wave)
+//   cover the latency, and two below: 8 items of 131072, dim 128, 101 [104 with two,
+//   113 with three]; 2 of 65536, dim 256, 40 [54]; 12 of 65536, dim 64, 45 [47 with
+//   one].
 extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
-  const int keys = a->dtype == RL_F32 ? 16 : 32;
+  const int size = a->dtype == RL_F32 ? 4 : 2;
+  const int keys = size == 4 ? 16 : 32;
   const long room = (long)a->cache.table_cols << a->cache.page_shift;
   const long most = (room + keys - 1) / keys;  // tiles of an item
   const int group = a->heads / a->kv_heads;
@@ -913,10 +1143,11 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
     a->waves = items >= 1024 ? 1 : 4;
     return;
   }
-  const long resident = (long)cus * (a->dim > 96 ? 1 : 2);
-  const long worth = (items * most + 3) / 4;  // a tile to each wave
-  a->workers = (int)(resident < worth ? resident : worth);
-  a->waves = 4;
+  a->waves = items >= 256 ? 1 : 4;
+  const int fit = resident_waves(a->dim, size);
+  const long fill = (long)cus * (a->waves == 1 ? 4 * (fit < 2 ? fit : 2) : a->dim > 96 ? 1 : 2);
+  const long worth = (items * most + a->waves - 1) / a->waves;  // a tile to each wave
+  a->workers = (int)(fill < worth ? fill : worth);
 }
 
 extern "C" int launch_paged_append(const PagedAppendArgs* a, void* stream) {
