@@ -387,10 +387,10 @@ PolicyLossArgs policy_args(const PolicyViews& v, const PolicyConfig& c) {
   a.log_high = std::log1p(c.high);
   a.log_low = c.low < 1 ? std::log1p(-c.low) : -INFINITY;
   a.log_off = std::log1p(c.low);
-  a.low = (float)(1 - c.low);
-  a.high = (float)(1 + c.high);
-  a.kl_coeff = (float)c.kl;
-  a.entropy_coeff = (float)c.entropy;
+  a.low = 1 - c.low;
+  a.high = 1 + c.high;
+  a.kl_coeff = c.kl;
+  a.entropy_coeff = c.entropy;
   a.mean = c.mean;
   return a;
 }

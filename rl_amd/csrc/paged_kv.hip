@@ -222,8 +222,8 @@ int append_vec(const PagedAppendArgs& a, hipStream_t st) {
 //
 // Measured (one MI355X, where a large copy runs at 4.9 TB/s): 1 x 131072 keys, 32 +
 // 8 heads of 128 bf16, 98 us a call, 93 in the kernel (5.8 TB/s) and 5 in the join;
-// 48 sequences of 1 to 8192 keys 157 us (5.1 TB/s); 256 of 65 to 96 keys, 12 heads of
-// 64, 14 us (4.6 TB/s).  Bound by HBM; small calls by three dependent loads (length,
+// 48 sequences of 1 to 8192 keys 152 us (5.3 TB/s); 256 of 65 to 96 keys, 12 heads of
+// 64, 13.5 us (4.7 TB/s).  Bound by HBM; small calls by three dependent loads (length,
 // page id, key) and the launch.
 // ---------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -262,19 +262,22 @@ struct SharedItem {
 };
 
 struct AttendPlan {
-  int workers;     // 0: one workgroup per item, nothing shared
+  int workers;     // 0: one worker per item, nothing shared
   int blocks;      // head blocks of 16 per key head
+  int group;       // query heads to a key head
+  int per;         // items of a sequence: kv_heads * blocks
   SharedItem* notes;  // [workers]
   float* part;     // [2 * workers][min(16, G)][dim] unnormalised outputs
   float* part_ms;  // [2 * workers][min(16, G)][2] maximum and sum
 };
 
-__device__ __forceinline__ int tiles_of(const PagedAttendArgs& a, long b, int tile) {
-  long len = whole(a.lengths, a.lengths_i64, b);
+__device__ __forceinline__ int length_of(const PagedAttendArgs& a, long b) {
+  const long len = whole(a.lengths, a.lengths_i64, b);
   const long room = (long)a.cache.table_cols << a.cache.page_shift;
-  len = len < room ? len : room;
-  return len > 0 ? (int)((len + tile - 1) / tile) : 1;
+  return (int)(len < 0 ? 0 : len < room ? len : room);
 }
+
+__device__ __forceinline__ int tiles_in(int len, int tile) { return len > 0 ? (len + tile - 1) / tile : 1; }
 
 // Where sequence `b` and its items lie on the line of all tiles.
 struct Spot {
@@ -293,7 +296,7 @@ struct Line {
 __device__ __forceinline__ void line_pass(const PagedAttendArgs& a, long per, int tile, long b0,
                                           Line& x) {
   const int lane = threadIdx.x & 63;
-  x.mine = b0 + lane < a.batch ? tiles_of(a, b0 + lane, tile) : 0;
+  x.mine = b0 + lane < a.batch ? tiles_in(length_of(a, b0 + lane), tile) : 0;
   x.upto = (long)x.mine * per;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -310,7 +313,7 @@ __device__ __forceinline__ Line line_of(const PagedAttendArgs& a, long per, int 
     return x;
   }
   long n = 0;
-  for (long b = threadIdx.x & 63; b < a.batch; b += 64) n += tiles_of(a, b, tile);
+  for (long b = threadIdx.x & 63; b < a.batch; b += 64) n += tiles_in(length_of(a, b), tile);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
   x.mine = 0;
@@ -663,14 +666,19 @@ struct Tiles<float, DP, EXACT> {
   __device__ __forceinline__ void turn_over() { ok = ok_next; }
 };
 
+// A place on the line of tiles.
+struct Cursor {
+  long b;
+  int item, at, tiles;  // at < tiles of the item
+  int len;              // of the sequence
+};
+
 template <typename T>
-__device__ __forceinline__ Item<T> item_of(const PagedAttendArgs& a, const AttendPlan& plan, long b,
-                                           int item) {
-  const int kv = item / plan.blocks;
-  const long room = (long)a.cache.table_cols << a.cache.page_shift;
-  const long len = whole(a.lengths, a.lengths_i64, b);
-  return {a.cache.table + b * a.cache.table_stride, (const T*)a.cache.k + kv * a.cache.k_head,
-          (const T*)a.cache.v + kv * a.cache.v_head, (int)(len < room ? len : room)};
+__device__ __forceinline__ Item<T> item_of(const PagedAttendArgs& a, const AttendPlan& plan,
+                                           const Cursor& c) {
+  const int kv = plan.blocks == 1 ? c.item : c.item / plan.blocks;
+  return {a.cache.table + c.b * a.cache.table_stride, (const T*)a.cache.k + kv * a.cache.k_head,
+          (const T*)a.cache.v + kv * a.cache.v_head, c.len};
 }
 
 // The first query head of an item and how many it has.
@@ -678,10 +686,10 @@ struct Heads {
   int first, count;
 };
 
-__device__ __forceinline__ Heads heads_of(const PagedAttendArgs& a, const AttendPlan& plan, int item) {
-  const int group = a.heads / a.kv_heads, kv = item / plan.blocks;
-  const int first = kv * group + 16 * (item % plan.blocks);
-  return {first, min(16, (kv + 1) * group - first)};
+__device__ __forceinline__ Heads heads_of(const AttendPlan& plan, int item) {
+  if (plan.blocks == 1) return {item * plan.group, plan.group};
+  const int kv = item / plan.blocks, block = item - kv * plan.blocks;
+  return {kv * plan.group + 16 * block, min(16, plan.group - 16 * block)};
 }
 
 template <typename W, typename T>
@@ -690,12 +698,6 @@ __device__ __forceinline__ typename W::Query query_of(const PagedAttendArgs& a, 
   const bool live = mine < h.count;
   return W::query((const T*)a.q + b * a.q_batch + (h.first + (live ? mine : 0)) * a.q_head, live, a.dim);
 }
-
-// A place on the line of tiles.
-struct Cursor {
-  long b;
-  int item, at, tiles;  // at < tiles of the item
-};
 
 // The range of the line that worker `me` takes, and its note for the join.
 struct Range {
@@ -706,27 +708,26 @@ struct Range {
 
 __device__ __forceinline__ Range range_of(const PagedAttendArgs& a, const AttendPlan& plan, int keys,
                                           int waves) {
-  const long me = blockIdx.x;
-  const int per = a.kv_heads * plan.blocks;
   Range x;
   x.note = {0, 0, 0, 0, 0};
-  if (plan.workers == 0) {
-    const long b = (unsigned)me / (unsigned)per;
-    const int tiles = tiles_of(a, b, keys);
-    x.from = {b, (int)(me - b * per), 0, tiles};
+  if (plan.workers == 0) {  // blockIdx: item, sequence
+    const int len = length_of(a, blockIdx.y), tiles = tiles_in(len, keys);
+    x.from = {(long)blockIdx.y, (int)blockIdx.x, 0, tiles, len};
     x.count = tiles;
     return x;
   }
+  const long me = blockIdx.x;
+  const int per = plan.per;
   const Line line = line_of(a, per, keys);
   const long busy = busy_workers(plan.workers, line.total, waves);
   x.count = 0;
-  x.from = {0, 0, 0, 1};
+  x.from = {0, 0, 0, 1, 0};
   if (me < busy) {
     const long lo = share(me, line.total, busy), hi = share(me + 1, line.total, busy);
     const Spot s = spot_of(a, per, keys, line, lo);
     const int item = (int)share(lo - s.first, 1, s.tiles);
     const int at = (int)(lo - s.first - (long)item * s.tiles);
-    x.from = {s.b, item, at, s.tiles};
+    x.from = {s.b, item, at, s.tiles, length_of(a, s.b)};
     x.count = (int)(hi - lo);
     if (at > 0) {
       // the first border strictly inside an item answers for its join
@@ -757,9 +758,7 @@ __global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_atten
   using W = Tiles<T, DP, EXACT>;
   __shared__ __attribute__((aligned(16))) char lds[sizeof(T) == 2 ? W::LDS_BYTES : 16];
   const int lane = threadIdx.x;
-  const int per = a.kv_heads * plan.blocks;
-  const int group = a.heads / a.kv_heads;
-  const int rows = group < 16 ? group : 16;
+  const int rows = plan.group < 16 ? plan.group : 16;
   const int shift = a.cache.page_shift;
   const Range range = range_of(a, plan, W::KEYS, 1);
   if (range.count == 0) return;
@@ -767,30 +766,35 @@ __global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_atten
   auto after = [&](Cursor c) {
     if (++c.at == c.tiles) {
       c.at = 0;
-      if (++c.item == per) {
+      if (++c.item == plan.per) {
         c.item = 0;
-        if (c.b + 1 < a.batch) c.tiles = tiles_of(a, ++c.b, W::KEYS);
+        if (c.b + 1 < a.batch) {
+          c.len = length_of(a, ++c.b);
+          c.tiles = tiles_in(c.len, W::KEYS);
+        }
       }
     }
     return c;
   };
-  Cursor now = range.from, next = after(now), far = after(next);
-  Item<T> it = item_of<T>(a, plan, now.b, now.item);
-  Heads heads = heads_of(a, plan, now.item);
+  Cursor now = range.from, next = now, far;
+  Item<T> it = item_of<T>(a, plan, now);
+  Heads heads = heads_of(plan, now.item);
   W w;
   typename W::Query q;
-  w.q = query_of<W, T>(a, now.b, heads);
-  w.clear();
   w.pages(it, shift, now.at);
+  w.q = query_of<W, T>(a, now.b, heads);
   w.resolve(a.cache, now.at);
   w.turn_over();
   const Item<T> first = it;
   if (range.count > 1) {
-    it = item_of<T>(a, plan, next.b, next.item);
+    next = after(now);
+    it = item_of<T>(a, plan, next);
     w.pages(it, shift, next.at);
   }
   w.fetch_k(first, a.dim);
   w.fetch_v(first, a.dim);
+  far = range.count > 2 ? after(next) : next;
+  w.clear();
   int begin = now.at;  // where this worker's part of the item begins
   long slot = 2 * (long)blockIdx.x;
   for (int i = 0; i < range.count; ++i) {
@@ -800,10 +804,10 @@ __global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_atten
     if (more) {
       w.resolve(a.cache, next.at);
       if (i + 2 < range.count) {
-        it = item_of<T>(a, plan, far.b, far.item);
+        it = item_of<T>(a, plan, far);
         w.pages(it, shift, far.at);  // ahead of the loads that follow
       }
-      if (last) q = query_of<W, T>(a, next.b, heads_of(a, plan, next.item));
+      if (last) q = query_of<W, T>(a, next.b, heads_of(plan, next.item));
     }
     w.scores(a.dim);
     if (more) w.fetch_k(ahead, a.dim);
@@ -838,7 +842,7 @@ __global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_atten
         }
       }
       if (more) {
-        heads = heads_of(a, plan, next.item);
+        heads = heads_of(plan, next.item);
         w.q = q;
         w.clear();
         begin = 0;
@@ -852,21 +856,18 @@ __global__ __launch_bounds__(64, resident_waves(DP, sizeof(T))) void paged_atten
   }
 }
 
-// Few items: the four waves of a workgroup share a worker's tiles and join what
-// they have at the end of each item.
-template <typename T, int DP, bool EXACT>
-__global__ __launch_bounds__(256, resident_waves(DP, sizeof(T))) void paged_attend_group_k(
+// Few items: the waves of a workgroup (four; one for short tables) share a worker's
+// tiles and join what they have at the end of each item.
+template <typename T, int DP, bool EXACT, int NW>
+__global__ __launch_bounds__(64 * NW, resident_waves(DP, sizeof(T))) void paged_attend_group_k(
     const PagedAttendArgs a, const AttendPlan plan) {
   using W = Tiles<T, DP, EXACT>;
-  constexpr int NW = 4;
   constexpr int OUT = DP + 4;  // pitch of a head's output in shared memory
   static_assert(16 * OUT * 4 <= W::LDS_BYTES, "the join reuses the staging rows");
   __shared__ __attribute__((aligned(16))) char lds[NW][W::LDS_BYTES];
   __shared__ float sm[NW][16], sl[NW][16];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
-  const int group = a.heads / a.kv_heads;
-  const int per = a.kv_heads * plan.blocks;  // items of a sequence
-  const int rows = group < 16 ? group : 16;
+  const int rows = plan.group < 16 ? plan.group : 16;
   const int shift = a.cache.page_shift;
   const Range range = range_of(a, plan, W::KEYS, NW);
   Cursor now = range.from;
@@ -874,15 +875,15 @@ __global__ __launch_bounds__(256, resident_waves(DP, sizeof(T))) void paged_atte
   bool first = true;
   while (left > 0) {
     const int end = left < now.tiles - now.at ? now.at + left : now.tiles;
-    const Item<T> it = item_of<T>(a, plan, now.b, now.item);
-    const Heads heads = heads_of(a, plan, now.item);
+    const Item<T> it = item_of<T>(a, plan, now);
+    const Heads heads = heads_of(plan, now.item);
     W w;
-    w.q = query_of<W, T>(a, now.b, heads);
-    w.clear();
     T* mine = (T*)lds[wave];
     int t = now.at + wave;
+    w.clear();
     if (t < end) {
       w.pages(it, shift, t);
+      w.q = query_of<W, T>(a, now.b, heads);
       w.resolve(a.cache, t);
       w.turn_over();
       if (t + NW < end) w.pages(it, shift, t + NW);
@@ -941,9 +942,10 @@ __global__ __launch_bounds__(256, resident_waves(DP, sizeof(T))) void paged_atte
     now.at = 0;
     if (left > 0) {
       __syncthreads();  // the rows above are staged into again
-      if (++now.item == per) {
+      if (++now.item == plan.per) {
         now.item = 0;
-        now.tiles = tiles_of(a, ++now.b, W::KEYS);
+        now.len = length_of(a, ++now.b);
+        now.tiles = tiles_in(now.len, W::KEYS);
       }
     }
   }
@@ -960,15 +962,12 @@ __global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs
   __shared__ f32x4 so[8][32];
   const SharedItem note = plan.notes[blockIdx.x];
   if (note.parts == 0) return;
-  const int group = a.heads / a.kv_heads;
-  const int rows = group < 16 ? group : 16;
-  const int kv = note.item / plan.blocks;
-  const int head0 = kv * group + 16 * (note.item % plan.blocks);
-  const int heads = min(16, (kv + 1) * group - head0);
+  const int rows = plan.group < 16 ? plan.group : 16;
+  const Heads heads = heads_of(plan, note.item);
   const int quads = a.dim / 4;
   const int half = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q = blockIdx.y * 32 + lane;
-  const int g = min(q / quads, heads - 1);  // lanes past the item repeat its last head
+  const int g = min(q / quads, heads.count - 1);  // lanes past the item repeat its last head
   const int quad = q % quads;
   float top = -INFINITY, sum = 0.f;
   f32x4 out = {0.f, 0.f, 0.f, 0.f};
@@ -1004,7 +1003,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs
   sl[half][lane] = sum;
   so[half][lane] = out;
   __syncthreads();
-  if (half != 0 || q >= heads * quads) return;
+  if (half != 0 || q >= heads.count * quads) return;
 #pragma unroll
   for (int o = 1; o < 8; ++o) top = fmaxf(top, sm[o][lane]);
   sum = 0.f;
@@ -1016,7 +1015,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs
     sum += f * sl[o][lane];
     out += f * so[o][lane];
   }
-  T* dst = (T*)a.out + (note.b * a.heads + head0 + g) * a.dim + 4 * quad;
+  T* dst = (T*)a.out + (note.b * a.heads + heads.first + g) * a.dim + 4 * quad;
 #pragma unroll
   for (int r = 0; r < 4; ++r) dst[r] = (T)(sum == 0.f ? 0.f : out[r] / sum);
 }
@@ -1026,14 +1025,13 @@ __global__ __launch_bounds__(256) void paged_attend_join_k(const PagedAttendArgs
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attend_join_few_k(const PagedAttendArgs a,
                                                                const AttendPlan plan) {
-  const int group = a.heads / a.kv_heads;
-  const int rows = group < 16 ? group : 16;
+  const int rows = plan.group < 16 ? plan.group : 16;
   const unsigned quads = a.dim / 4, all = rows * quads;
   const unsigned id = blockIdx.x * 256 + threadIdx.x;
   if (id / all >= (unsigned)plan.workers) return;
   const SharedItem note = plan.notes[id / all];
   const int g = (int)(id % all / quads), quad = (int)(id % quads);
-  const Heads heads = heads_of(a, plan, note.item);
+  const Heads heads = heads_of(plan, note.item);
   if (note.parts == 0 || g >= heads.count) return;
   float top = -INFINITY, sum = 0.f;
   f32x4 out = {0.f, 0.f, 0.f, 0.f};
@@ -1071,16 +1069,24 @@ __global__ __launch_bounds__(256) void paged_attend_join_few_k(const PagedAttend
 
 template <typename T, int DP, bool EXACT>
 void attend_kernel(const PagedAttendArgs& a, const AttendPlan& plan, hipStream_t st) {
-  const dim3 blocks((unsigned)(a.workers ? a.workers : a.batch * a.kv_heads * a.head_blocks));
-  if (a.waves == 1)
-    hipLaunchKernelGGL((paged_attend_wave_k<T, DP, EXACT>), blocks, dim3(64), 0, st, a, plan);
-  else
-    hipLaunchKernelGGL((paged_attend_group_k<T, DP, EXACT>), blocks, dim3(256), 0, st, a, plan);
+  if (a.workers == 0) {
+    const dim3 items(plan.per, (unsigned)a.batch);
+    if (a.waves == 1)
+      hipLaunchKernelGGL((paged_attend_group_k<T, DP, EXACT, 1>), items, dim3(64), 0, st, a, plan);
+    else
+      hipLaunchKernelGGL((paged_attend_group_k<T, DP, EXACT, 4>), items, dim3(256), 0, st, a, plan);
+  } else if (a.waves == 1) {
+    hipLaunchKernelGGL((paged_attend_wave_k<T, DP, EXACT>), dim3(a.workers), dim3(64), 0, st, a, plan);
+  } else {
+    hipLaunchKernelGGL((paged_attend_group_k<T, DP, EXACT, 4>), dim3(a.workers), dim3(256), 0, st, a,
+                       plan);
+  }
 }
 
 template <typename T>
 int attend_any(const PagedAttendArgs& a, hipStream_t st) {
-  const AttendPlan plan{a.workers, a.head_blocks, (SharedItem*)a.notes, a.part, a.part_ms};
+  const AttendPlan plan{a.workers, a.head_blocks, a.heads / a.kv_heads, a.kv_heads * a.head_blocks,
+                        (SharedItem*)a.notes, a.part, a.part_ms};
   if (a.dim < 64)
     attend_kernel<T, 64, false>(a, plan, st);
   else if (a.dim == 64)
@@ -1098,8 +1104,7 @@ int attend_any(const PagedAttendArgs& a, hipStream_t st) {
   else
     attend_kernel<T, 256, true>(a, plan, st);
   if (a.workers < 2) return (int)hipGetLastError();
-  const int group = a.heads / a.kv_heads;
-  const long quads = (long)(group < 16 ? group : 16) * (a.dim / 4);
+  const long quads = (long)(plan.group < 16 ? plan.group : 16) * (a.dim / 4);
   if (a.waves == 1)
     hipLaunchKernelGGL((paged_attend_join_few_k<T>), dim3((unsigned)((a.workers * quads + 255) / 256)),
                        dim3(256), 0, st, a, plan);
@@ -1138,7 +1143,8 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   const int group = a->heads / a->kv_heads;
   a->head_blocks = (group + 15) / 16;
   const long items = a->batch * a->kv_heads * a->head_blocks;
-  if (most <= 8 || (most <= 16 && items >= 1024)) {
+  // (a grid's y takes 65535 sequences)
+  if ((most <= 8 || (most <= 16 && items >= 1024)) && a->batch < 65536) {
     a->workers = 0;
     a->waves = items >= 1024 ? 1 : 4;
     return;

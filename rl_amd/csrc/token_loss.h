@@ -49,7 +49,7 @@ struct PolicyLossArgs {
   double log_low, log_high;    // borders of the log ratio
   double log_off;              // upper border of the clip_fraction count
   float low, high;             // the clipped ratio's values: 1 - low, 1 + high
-  float kl_coeff, entropy_coeff;
+  double kl_coeff, entropy_coeff;
   int mean;                // 1: divide by the mask's sum, 0: plain sums
   double* partials;        // [blocks][8]
   int blocks;

@@ -402,10 +402,10 @@ int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
 //   entropy term: + lp (the sampled estimate of -H); d/dlp = 1
 //   objective = -sum w gain / D, and the rest likewise
 //
-// Whether a ratio is clipped is decided on x against the borders' logarithms,
-// in double where float32 could fall on the other side, so that an element next
-// to a border is treated as in the definition.  e^y - 1 - y cancels near 0: a
-// series there.  Four tokens are summed in float32, what follows in double.
+// Whether a ratio is clipped is decided in double on x against the borders'
+// logarithms, so that an element next to a border is treated as in the definition.
+// e^y - 1 - y cancels near 0: a series there.  Sums are in double throughout: gains
+// of either sign cancel, and the loop has the time.
 //
 // One workgroup does everything up to 16K tokens (two launches cost more than
 // its few passes); above, partial sums of many and a second launch that joins
@@ -456,27 +456,20 @@ __device__ __forceinline__ float kl3(float y) {
 }
 
 struct PolicyToken {
-  bool above, below, off;
-  float x, ratio;
+  bool above, below;
+  double x, ratio;
 };
 
+// The ratio e^x.  Near 1, where policies are, as 1 + x + (e^x - 1 - x) with the
+// sums in double: sums of signed gains cancel, and an exponential's last bit would
+// show in them.  Further off the instruction's 1 ulp.
 __device__ __forceinline__ PolicyToken policy_token(const PolicyLossArgs& a, float lp, float old) {
   PolicyToken t;
-  t.x = lp - old;
-  const float lo = (float)a.log_low, hi = (float)a.log_high, off = (float)a.log_off;
-  t.above = t.x > hi;
-  t.below = t.x < lo;
-  t.off = t.x > off;
-  // the difference and the borders are each rounded once: 2^-21 is 4 times that
-  const float near = 4.76837158e-7f * fmaxf(1.f, fabsf(t.x));
-  if (fabsf(t.x - hi) < near || fabsf(t.x - lo) < near || fabsf(t.x - off) < near) {
-    const double x = (double)lp - (double)old;
-    t.above = x > a.log_high;
-    t.below = x < a.log_low;
-    t.off = x > a.log_off;
-  }
-  t.off = t.off || t.below;
-  t.ratio = exp2_hw(t.x * kLog2e);
+  t.x = (double)lp - (double)old;
+  t.above = t.x > a.log_high;
+  t.below = t.x < a.log_low;
+  const float x = (float)t.x;
+  t.ratio = fabsf(x) <= 0.5f ? 1.0 + (t.x + (double)kl3(x)) : (double)exp2_hw(x * kLog2e);
   return t;
 }
 
@@ -486,21 +479,21 @@ __device__ __forceinline__ bool clipped_against(const PolicyToken& t, float adv)
 
 enum { S_GAIN, S_KL, S_LP, S_W, S_R, S_RR, S_OFF, S_COUNT };
 
-// One token's terms, added to float sums of a few tokens.
+// One token's terms.
 __device__ __forceinline__ void policy_terms(const PolicyLossArgs& a, float lp, float old, float adv,
-                                             float w, float ref, bool has_ref, float (&s)[S_COUNT]) {
+                                             float w, float ref, bool has_ref, double (&s)[S_COUNT]) {
   const PolicyToken t = policy_token(a, lp, old);
   s[S_R] += t.ratio;
   s[S_RR] += t.ratio * t.ratio;
-  s[S_OFF] += t.off ? 1.f : 0.f;
+  s[S_OFF] += t.x > a.log_off || t.below ? 1.0 : 0.0;
   if (w == 0.f) return;  // a masked token may hold anything, NaN too
-  const float bound = t.above ? a.high : t.below ? a.low : t.ratio;
-  const float gain = a.variant == 0 ? (clipped_against(t, adv) ? bound : t.ratio) * adv
-                                    : bound * t.x * adv;
+  const double bound = t.above ? a.high : t.below ? a.low : t.ratio;
+  const double gain = a.variant == 0 ? (clipped_against(t, adv) ? bound : t.ratio) * adv
+                                     : bound * t.x * adv;
   s[S_GAIN] += w * gain;
   s[S_W] += w;
-  s[S_LP] += w * lp;
-  if (has_ref) s[S_KL] += w * kl3(ref - lp);
+  s[S_LP] += (double)w * lp;
+  if (has_ref) s[S_KL] += (double)w * kl3(ref - lp);
 }
 
 // What a token's gradient is, before its upstream factors are folded in:
@@ -510,8 +503,9 @@ __device__ __forceinline__ float policy_grad(const PolicyLossArgs& a, float lp, 
                                              float ge) {
   if (w == 0.f) return 0.f;
   const PolicyToken t = policy_token(a, lp, old);
-  const float dgain = a.variant == 0 ? (clipped_against(t, adv) ? 0.f : t.ratio * adv)
-                                     : (t.above ? a.high : t.below ? a.low : t.ratio) * adv;
+  const float ratio = (float)t.ratio;
+  const float dgain = a.variant == 0 ? (clipped_against(t, adv) ? 0.f : ratio * adv)
+                                     : (float)(t.above ? a.high : t.below ? a.low : t.ratio) * adv;
   float d = ge - go * dgain;
   if (has_ref) {
     const float y = ref - lp;
@@ -626,13 +620,10 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_dense_fwd_k(const PolicyLos
   for (unsigned i = 4 * (blockIdx.x * BLOCK + threadIdx.x); i < n; i += 4 * gridDim.x * BLOCK) {
     Four f;
     load_four<T>(a, i, n, f);
-    float part[S_COUNT] = {};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (i + k < n)
-        policy_terms(a, f.lp[k], f.old[k], f.adv[k], f.w[k], has_ref ? f.ref[k] : 0.f, has_ref, part);
-#pragma unroll
-    for (int k = 0; k < S_COUNT; ++k) s[k] += part[k];
+        policy_terms(a, f.lp[k], f.old[k], f.adv[k], f.w[k], has_ref ? f.ref[k] : 0.f, has_ref, s);
   }
   if (!block_sums<BLOCK>(s)) return;
   if (gridDim.x == 1) {
@@ -650,12 +641,9 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_fwd_k(const PolicyLossArgs 
   const bool has_ref = a.ref.ptr != nullptr;
   for (long i = (long)blockIdx.x * BLOCK + threadIdx.x; i < n; i += (long)gridDim.x * BLOCK) {
     const long r = n < (1L << 31) ? row_of(a, (unsigned)i) : i / a.cols, c = i - r * a.cols;
-    float part[S_COUNT] = {};
     policy_terms(a, operand(a.log_probs, r, c), operand(a.old_log_probs, r, c),
                  operand(a.advantage, r, c), a.mask.ptr ? operand(a.mask, r, c) : 1.f,
-                 has_ref ? operand(a.ref, r, c) : 0.f, has_ref, part);
-#pragma unroll
-    for (int k = 0; k < S_COUNT; ++k) s[k] += part[k];
+                 has_ref ? operand(a.ref, r, c) : 0.f, has_ref, s);
   }
   if (!block_sums<BLOCK>(s)) return;
   if (gridDim.x == 1) {
@@ -682,8 +670,8 @@ __device__ __forceinline__ PolicyUpstream policy_upstream(const PolicyLossArgs& 
   const float inv = *a.scale;
   const float total = a.g_total ? *a.g_total : 0.f;
   return {(total + (a.g_objective ? *a.g_objective : 0.f)) * inv,
-          (total + (a.g_kl ? *a.g_kl : 0.f)) * a.kl_coeff * inv,
-          (total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv};
+          (float)((total + (a.g_kl ? *a.g_kl : 0.f)) * a.kl_coeff * inv),
+          (float)((total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv)};
 }
 
 template <typename T>
