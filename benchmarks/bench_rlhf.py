@@ -28,6 +28,8 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
+from rl_amd import ops  # noqa: E402
+
 
 def build_gpt2_small(device, attn: str = "sdpa"):
     from transformers import GPT2Config, GPT2LMHeadModel
@@ -50,11 +52,13 @@ def main():
     p.add_argument("--prompt-len", type=int, default=64)
     p.add_argument("--gen-len", type=int, default=32)
     p.add_argument("--decode-mode",
-                   choices=["generate", "manual", "graphdec", "static",
-                            "graph"],
+                   choices=["generate", "manual", "graphdec", "paged",
+                            "static", "graph"],
                    default="graphdec",
-                   help="HF generate (default) / eager static-KV loop / "
-                        "hipGraph-captured loop.  static and graph SEGFAULT on "
+                   help="HF generate / eager static-KV loop / "
+                        "hipGraph-captured loop (default) / paged cache, "
+                        "with behavior log-probs from the rollout and the "
+                        "fused log-prob and policy-loss operators.  static and graph SEGFAULT on "
                         "this stack (ROCm 7.2 + transformers 5.15 GPT2 "
                         "StaticCache decode, with both sdpa and eager "
                         "attention) — kept opt-in for newer stacks")
@@ -87,9 +91,15 @@ def main():
     autocast = torch.autocast("cuda", dtype=torch.bfloat16, enabled=cuda, cache_enabled=False)
     kl_coef, clip_eps = 0.05, 0.2
 
+    fused = args.decode_mode == "paged"
+
     def token_log_probs(model, ids, mask):
         out = model.transformer(input_ids=ids, attention_mask=mask)
         hidden = out.last_hidden_state
+        if fused:
+            # only the response's rows reach the LM head
+            logits = model.lm_head(hidden[:, P - 1 : -1])
+            return ops.token_log_probs(logits, ids[:, P:]), hidden
         logits = model.lm_head(hidden)
         lp = logits[:, P - 1 : -1].log_softmax(-1)
         resp = ids[:, P:]
@@ -172,6 +182,16 @@ def main():
             print("graphdec capture failed; eager decode body stays",
                   file=sys.stderr)
 
+    pageddec = None
+    if fused:
+        from rl_amd.modules.llm import PagedGPT2Decoder
+
+        pageddec = PagedGPT2Decoder(policy, B, P + G, device)
+        pageddec.prefill(torch.randint(0, V, (B, P), device=device))
+        if not pageddec.capture():
+            print("paged capture failed; eager decode body stays",
+                  file=sys.stderr)
+
     def manual_rollout(prompts):
         """Hand-rolled sampling loop over the ordinary dynamic KV cache
         (the same cache `generate` uses — StaticCache segfaults on this
@@ -196,7 +216,10 @@ def main():
     def one_iteration():
         prompts = torch.randint(0, V, (B, P), device=device)
         mask = torch.ones_like(prompts)
-        if graphdec is not None:
+        if pageddec is not None:
+            rolled = pageddec.rollout(prompts, G)
+            gen = torch.cat([prompts, rolled.get("tokens_response")], 1)
+        elif graphdec is not None:
             gen = graphdec.rollout(prompts, G)
         elif args.decode_mode == "manual":
             gen = manual_rollout(prompts)
@@ -223,7 +246,10 @@ def main():
                 )
         full_mask = torch.ones_like(gen)
         with torch.no_grad(), autocast:
-            old_lp, _ = token_log_probs(policy, gen, full_mask)
+            if fused:
+                old_lp = rolled.get("log_probs")
+            else:
+                old_lp, _ = token_log_probs(policy, gen, full_mask)
             ref_lp, _ = token_log_probs(ref, gen, full_mask)
         # synthetic scalar reward per sequence (stand-in for a reward model)
         reward = (gen[:, P:] % 97).float().mean(-1, keepdim=True) / 97.0
@@ -233,14 +259,19 @@ def main():
             # sequence-level advantage broadcast over tokens (GRPO-style
             # whitening across the batch)
             adv = (reward - reward.mean()) / reward.std().clamp_min(1e-4)
-            ratio = (new_lp - old_lp).exp()
-            g1 = ratio * adv
-            g2 = ratio.clamp(1 - clip_eps, 1 + clip_eps) * adv
-            pg_loss = -torch.minimum(g1, g2).mean()
             v_loss = 0.5 * (values - reward).pow(2).mean()
-            lr_ = ref_lp - new_lp
-            kl = (lr_.exp() - 1 - lr_).mean()  # k3 estimator
-            loss = pg_loss + v_loss + kl_coef * kl
+            if fused:
+                loss = v_loss + ops.token_policy_loss(
+                    new_lp, old_lp, adv, None, ref_lp, clip_low=clip_eps,
+                    clip_high=clip_eps, kl_coeff=kl_coef).loss_total
+            else:
+                ratio = (new_lp - old_lp).exp()
+                g1 = ratio * adv
+                g2 = ratio.clamp(1 - clip_eps, 1 + clip_eps) * adv
+                pg_loss = -torch.minimum(g1, g2).mean()
+                lr_ = ref_lp - new_lp
+                kl = (lr_.exp() - 1 - lr_).mean()  # k3 estimator
+                loss = pg_loss + v_loss + kl_coef * kl
         optim.zero_grad(set_to_none=True)
         loss.backward()
         if distributed:
@@ -254,6 +285,8 @@ def main():
                 g.copy_(flat[i : i + g.numel()].reshape(g.shape))
                 i += g.numel()
         optim.step()
+        if pageddec is not None:
+            pageddec.refresh_weights()
         if graphdec is not None:
             graphdec.refresh_weights()
 
@@ -300,7 +333,8 @@ def main():
                         "parallelism": f"dp{world}",
                         "kl_to_ref": "k3",
                         "decode": ("graph" if decode_graph is not None
-                                   else "static" if use_static else "generate"),
+                                   else "static" if use_static
+                                   else "paged" if fused else "generate"),
                     },
                 }
             )

@@ -250,7 +250,25 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         self.gen_buf = torch.zeros(batch, max_len, dtype=torch.long, device=device)
         self.lp_buf = torch.zeros(batch, max_len, dtype=torch.float32, device=device)
         self.mask_buf = torch.zeros(batch, max_len, dtype=torch.bool, device=device)
+        # the sampling scores, padded so that an argmax goes in two short stages
+        self._chunks = -(-self.V // self._CHUNK)
+        self._scores = torch.full((batch, self._chunks * self._CHUNK), float("-inf"), device=device)
         self._graph = None
+
+    _CHUNK = 512
+
+    def _draw(self, logits: torch.Tensor) -> torch.Tensor:
+        """A token of ``softmax(logits / temperature)`` per row: the argmax of
+        ``logits / temperature - log(e)`` with ``e`` exponential.  (Not
+        ``multinomial``: its validity checks reduce the whole tensor over many
+        blocks, which puts memory-set nodes into a captured graph, and those
+        have given wrong results on later replays; short rows are reduced
+        without them.)"""
+        noise = torch.empty_like(logits).exponential_().log_()
+        torch.sub(logits / self.temperature, noise, out=self._scores[:, : self.V])
+        best, at = self._scores.view(self.B, self._chunks, self._CHUNK).max(-1)
+        chunk = best.argmax(-1, keepdim=True)
+        return (chunk * self._CHUNK + at.gather(1, chunk)).squeeze(-1)
 
     def _step_logits(self) -> torch.Tensor:
         """One decode forward: ``[B, V]`` fp32 logits after the tokens in
@@ -282,7 +300,7 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         """Sample the next token of every sequence and record it; stopped
         sequences record the end token outside the mask."""
         on = self.active.bool()
-        nxt = torch.multinomial(torch.softmax(logits / self.temperature, -1), 1).squeeze(-1)
+        nxt = self._draw(logits)
         if self.eos_token_id is not None:
             nxt = torch.where(on, nxt, self.eos_token_id)
         lp = ops.token_log_probs(logits, torch.where(on, nxt, -100), temperature=self.temperature)

@@ -203,6 +203,25 @@ def test_paged_rollout_stops_at_the_end_token(device):
     assert (lp.double() - want).abs().max() < 2e-4
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_paged_rollout_draws_from_the_distribution(device):
+    """40000 draws over 1500 tokens (three chunks) from six likely ones; each
+    count is within 5 standard deviations, and no masked token is drawn."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm(vocab_size=1500).to(device)
+    dec = PagedGPT2Decoder(model, 400, 8, device, dtype=torch.float32, temperature=2.0)
+    logits = torch.full((1500,), -math.inf)
+    likely = torch.tensor([0, 511, 512, 1023, 1024, 1499])
+    logits[likely] = torch.tensor([0.0, 1.0, 2.0, 3.0, 1.0, -1.0])
+    p = torch.softmax(logits[likely].double() / 2.0, 0)
+    rows = logits.expand(400, -1).contiguous().to(device)
+    torch.manual_seed(0)
+    counts = sum(torch.bincount(dec._draw(rows).cpu(), minlength=1500) for _ in range(100))
+    assert int(counts[likely].sum()) == 40000
+    assert ((counts[likely] - 40000 * p).abs() <= 5 * (40000 * p * (1 - p)).sqrt()).all()
+
+
 def test_paged_rollout_refusals():
     from rl_amd.modules.llm import PagedGPT2Decoder
 
@@ -515,3 +534,34 @@ def test_log_probs_past_32_bits():
     assert abs(float(grad[-1, 5]) - (1 - math.exp(3.0) / s)) < 2.0 ** -8
     assert abs(float(grad[-1, 6]) + 1 / s) < 2.0 ** -8 / s
     assert abs(float(grad[-2, -1]) + 1 / vocab) < 2.0 ** -8 / vocab
+
+
+@pytest.mark.gpu
+def test_rlhf_iterations_bf16():
+    """Rollouts by graph replay between optimizer steps: after every update the
+    recorded log-probs are those of the updated model (bf16 against fp32: the
+    logits of size 1 differ by some 2^-8 per layer), and everything stays finite."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm(n_head=2, vocab_size=5003).cuda()
+    optim = torch.optim.AdamW(model.parameters(), lr=1e-4)
+    dec = PagedGPT2Decoder(model, 64, 48, "cuda")
+    g = torch.Generator().manual_seed(0)
+    for it in range(5):
+        prompts = torch.randint(0, 5003, (64, 16), generator=g).cuda()
+        if it == 0:
+            dec.prefill(prompts)
+            assert dec.capture()
+        out = dec.rollout(prompts, 32)
+        ids = torch.cat([prompts, out.get("tokens_response")], 1)
+        assert (ids >= 0).all() and (ids < 5003).all()
+        with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+            logits = model(ids).logits[:, 15:-1]
+        lp = ops.token_log_probs(logits, ids[:, 16:])
+        assert (lp.detach() - out.get("log_probs")).abs().max() < 0.15
+        loss = ops.token_policy_loss(lp, out.get("log_probs"), torch.randn(64, 1, generator=g).cuda())
+        optim.zero_grad()
+        loss.loss_total.backward()
+        assert all(p.grad.isfinite().all() for p in model.parameters())
+        optim.step()
+        dec.refresh_weights()
