@@ -76,8 +76,9 @@ void token_log_probs_check(const Tensor& logits, const Tensor& tokens, double te
                     tokens.sizes(), " for logits ", logits.sizes());
   TORCH_CHECK_VALUE(logits.size(-1) >= 1 && logits.size(-1) <= INT32_MAX, op,
                     ": the vocabulary must hold 1 to 2**31 - 1 tokens, got ", logits.size(-1));
-  TORCH_CHECK_VALUE(std::isfinite(temperature) && temperature > 0, op,
-                    ": temperature must be positive and finite, got ", temperature);
+  // its reciprocal times log2(e) has to be a float32
+  TORCH_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e30, op,
+                    ": temperature must be positive and within 1e-30 to 1e30, got ", temperature);
   same_device(logits, tokens, op, "tokens");
 }
 
@@ -195,6 +196,12 @@ void paged_kv_append_check(const Tensor& k, const Tensor& v, const Tensor& k_cac
   }
   no_grad(op, k_cache, "k_cache");
   no_grad(op, v_cache, "v_cache");
+  TORCH_CHECK_VALUE(k_cache.data_ptr() != v_cache.data_ptr() || k_cache.data_ptr() == nullptr, op,
+                    ": k_cache and v_cache are the same memory");
+  for (const Tensor* t : {&k_cache, &v_cache})
+    for (int d = 0; d < 3; ++d)
+      TORCH_CHECK_VALUE(t->size(d) == 1 || t->stride(d) != 0, op,
+                        ": a cache that is written must not be expanded");
   TORCH_CHECK_VALUE(batch * k.size(1) <= kMostBlocks, op, ": at most ", kMostBlocks,
                     " tokens in one call, got ", batch * k.size(1));
   per_sequence(op, start, "start", batch, k_cache);
@@ -530,7 +537,7 @@ PagedCache cache_of(const Tensor& k, const Tensor& v, const Tensor& table) {
 Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
 bool aligned_rows(const Tensor& t, int64_t wide) {
-  bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % (wide * t.element_size()) == 0;
   for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.size(d) == 1 || t.stride(d) % wide == 0);
   return ok;
 }
@@ -565,15 +572,12 @@ OptTensor paged_kv_append(const Tensor& k_in, const Tensor& v_in, const Tensor& 
   a.dim = (int)k.size(3);
   a.dtype = code_of(k, "paged_kv_append");
   a.interleaved = interleaved;
-  const int64_t wide = 16 / k.element_size();
-  bool vec = aligned_rows(k, wide) && aligned_rows(v, wide);
   if (rope) {
     const Tensor& cos = std::get<0>(*rope);
     a.cos = cos.data_ptr<float>();
     a.sin = std::get<1>(*rope).data_ptr<float>();
     a.positions = cos.size(0);
     a.rotary = 2 * (int)cos.size(1);
-    vec = vec && cos.size(1) % wide == 0;
   }
   if (q_in) {
     q = dense_last(*q_in);
@@ -582,9 +586,14 @@ OptTensor paged_kv_append(const Tensor& k_in, const Tensor& v_in, const Tensor& 
     a.heads = (int)q.size(2);
     q_out = torch::empty(q.sizes(), q.options());
     a.q_out = q_out.data_ptr();
-    vec = vec && aligned_rows(q, wide);
   }
-  a.vec = vec ? (int)wide : 1;
+  // the widest access, up to 16 bytes, that addresses and rotation halves allow
+  a.vec = (int)(16 / k.element_size());
+  auto fits = [&](int64_t wide) {
+    return aligned_rows(k, wide) && aligned_rows(v, wide) && (!q_in || aligned_rows(q, wide)) &&
+           a.rotary / 2 % wide == 0;
+  };
+  while (a.vec > 1 && !fits(a.vec)) a.vec = a.vec > 4 ? 4 : 1;
   if (a.batch * a.width) launched(launch_paged_append(&a, stream_of()), "paged_kv_append");
   return q_in ? OptTensor(q_out) : std::nullopt;
 }

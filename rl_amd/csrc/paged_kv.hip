@@ -182,6 +182,7 @@ int append_launch(const PagedAppendArgs& a, hipStream_t st) {
 template <typename T, int WIDE>
 int append_vec(const PagedAppendArgs& a, hipStream_t st) {
   if (a.vec >= WIDE) return append_launch<T, WIDE>(a, st);
+  if (a.vec >= 4) return append_launch<T, 4>(a, st);
   return append_launch<T, 1>(a, st);
 }
 

@@ -238,6 +238,11 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         if max_len > model.config.n_positions:
             raise ValueError(
                 f"PagedGPT2Decoder: max_len {max_len} exceeds the model's {model.config.n_positions} positions")
+        if eos_token_id is not None and not 0 <= eos_token_id < model.config.vocab_size:
+            raise ValueError(
+                f"PagedGPT2Decoder: eos_token_id {eos_token_id} is not in the vocabulary of {model.config.vocab_size}")
+        if not 1e-30 <= temperature <= 1e30:
+            raise ValueError(f"PagedGPT2Decoder: temperature must be positive, got {temperature}")
         self._bind(model, batch, max_len, device, dtype)
         self.temperature = temperature
         self.eos_token_id = eos_token_id

@@ -113,7 +113,8 @@ class GRPOLoss(LossModule):
         ):
             return None
         variant, low, high = self._fused_clip()
-        if not all(isinstance(x, (int, float)) and x >= 0 for x in (low, high)):
+        coeffs = (low, high, self.entropy_coeff or 0.0, self.kl_to_ref_coeff or 0.0)
+        if not all(isinstance(x, (int, float)) for x in coeffs) or low < 0 or high < 0:
             return None
         loss = ops.token_policy_loss(
             new_lp, old_lp, adv, mask, ref_lp, clip_low=low, clip_high=high, variant=variant,

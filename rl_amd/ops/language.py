@@ -34,12 +34,10 @@ __all__ = [
 _VARIANTS = {"clip": 0, "cispo": 1}
 
 
-def _ext(tensor: torch.Tensor):
-    """The extension for a tensor: required on the GPU, its argument checks
-    used on the CPU where it is built."""
-    if tensor.is_cuda:
-        _require_ext()
-    return _C
+def _native(tensor: torch.Tensor):
+    """The extension for a GPU tensor; None on the CPU (and on a GPU without
+    it where the eager fallback is allowed)."""
+    return _C if tensor.is_cuda and _require_ext() else None
 
 
 # --------------------------------------------------------------------------- #
@@ -62,7 +60,7 @@ def token_log_probs(
             do not count: their log-prob is 0, their logits are not read and
             get a gradient of exactly 0.  Any other token outside ``[0, V)``
             gives NaN (nothing is read out of range).
-        temperature: positive and finite.
+        temperature: positive (1e-30 to 1e30).
 
     Returns:
         ``[...]`` float32.  Differentiable in ``logits`` (once); the gradient
@@ -70,16 +68,19 @@ def token_log_probs(
         gradient of exactly 0 whatever its logits hold.  A row of nothing but
         ``-inf`` gives NaN.
     """
-    c = _ext(logits)
-    if logits.is_cuda:
-        return c.token_log_probs(logits, tokens, temperature, ignore_index)
+    c = _native(logits)
     if c is not None:
-        c.token_log_probs_check(logits, tokens, temperature)
-    known = (tokens >= 0) & (tokens < logits.shape[-1]) & (tokens != ignore_index)
+        return c.token_log_probs(logits, tokens, temperature, ignore_index)
+    if _C is not None:
+        _C.token_log_probs_check(logits, tokens, temperature)
+    gone = tokens == ignore_index
+    known = (tokens >= 0) & (tokens < logits.shape[-1])
     at = torch.where(known, tokens, 0).long().unsqueeze(-1)
-    lp = (logits.float() / temperature).log_softmax(-1).gather(-1, at).squeeze(-1)
-    lp = torch.where(known, lp, torch.nan)
-    return torch.where(tokens == ignore_index, 0.0, lp)
+    # ignored rows are replaced first: a NaN there would come back through the
+    # backward pass as 0 * NaN
+    x = torch.where(gone.unsqueeze(-1), 0.0, logits.float() / temperature)
+    lp = torch.where(known, x.log_softmax(-1).gather(-1, at).squeeze(-1), torch.nan)
+    return torch.where(gone, 0.0, lp)
 
 
 # --------------------------------------------------------------------------- #
@@ -144,13 +145,13 @@ def token_policy_loss(
         raise ValueError(f"token_policy_loss: variant must be one of {sorted(_VARIANTS)}, got {variant!r}")
     if reduction not in ("mean", "sum"):
         raise ValueError(f"token_policy_loss: reduction must be 'mean' or 'sum', got {reduction!r}")
-    c = _ext(log_probs)
-    if log_probs.is_cuda:
+    c = _native(log_probs)
+    if c is not None:
         return TokenPolicyLoss(*c.token_policy_loss(
             log_probs, old_log_probs, advantage, mask, ref_log_probs, _VARIANTS[variant],
             clip_low, clip_high, kl_coeff, entropy_coeff, reduction == "mean"))
-    if c is not None:
-        c.token_policy_loss_check(
+    if _C is not None:
+        _C.token_policy_loss_check(
             log_probs, old_log_probs, advantage, mask, ref_log_probs,
             clip_low, clip_high, kl_coeff, entropy_coeff)
     lp, old = log_probs.float(), old_log_probs.float()
@@ -250,17 +251,18 @@ def paged_kv_append(
 
     A token whose position is negative or past the table's columns, or whose
     page id is outside ``[0, pages)``, is not written.  A position past the
-    rotation's table gives NaN.  Two tokens of one call must not share a slot.
+    rotation's table gives NaN.  Two tokens of one call must not share a slot, and
+    ``k`` and ``v`` must not lie in the caches.
 
     Returns:
         The rotated queries (dense; zeros where padding), or None without ``q``.
     """
-    c = _ext(k_cache)
-    if k_cache.is_cuda:
+    c = _native(k_cache)
+    if c is not None:
         return c.paged_kv_append(
             k, v, k_cache, v_cache, page_table, start, lengths, q, rope, interleaved)
-    if c is not None:
-        c.paged_kv_append_check(k, v, k_cache, v_cache, page_table, start, lengths, q, rope)
+    if _C is not None:
+        _C.paged_kv_append_check(k, v, k_cache, v_cache, page_table, start, lengths, q, rope)
     batch, width = k.shape[:2]
     page_size = k_cache.shape[2]
     step = torch.arange(width, device=k.device)
@@ -313,13 +315,13 @@ def paged_attention_decode(
     Returns:
         ``[batch, heads, dim]`` in ``q``'s dtype.
     """
-    c = _ext(q)
-    if q.is_cuda:
+    c = _native(q)
+    if c is not None:
         return c.paged_attention_decode(q, k_cache, v_cache, page_table, lengths, scale)
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, q.shape[-1]))
-    if c is not None:
-        c.paged_attention_check(q, k_cache, v_cache, page_table, lengths, scale)
+    if _C is not None:
+        _C.paged_attention_check(q, k_cache, v_cache, page_table, lengths, scale)
     batch, heads, dim = q.shape
     kv_heads, page_size = k_cache.shape[1], k_cache.shape[2]
     if not page_table.shape[1]:

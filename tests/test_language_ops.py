@@ -154,6 +154,19 @@ def test_log_probs_masked_vocabulary(device, dtype, vocab):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_ignored_rows_pass_nothing_back(device):
+    logits = torch.randn(3, 2, 40, generator=gen(1))
+    logits[1, 0] = math.nan
+    logits[2] = math.inf
+    logits = logits.to(device).requires_grad_()
+    tokens = torch.tensor([[3, 39], [7, 0], [7, 7]], device=device)
+    lp = ops.token_log_probs(logits, tokens, ignore_index=7)
+    (grad,) = torch.autograd.grad(lp.sum(), logits)
+    assert (lp[tokens == 7] == 0).all() and lp.isfinite().all()
+    assert (grad[tokens == 7] == 0).all() and grad.isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_log_probs_tokens_out_of_range(device):
     logits = torch.randn(4, 9, generator=gen(0)).to(device)
     tokens = torch.tensor([-1, 9, 2 ** 40, 3], device=device)
@@ -203,7 +216,7 @@ def test_log_probs_refusals(device):
         ops.token_log_probs(logits, tokens[:1])
     with pytest.raises(ValueError, match="vocabulary"):
         ops.token_log_probs(logits[:, :0], tokens)
-    for bad in (0.0, -1.0, math.inf, math.nan):
+    for bad in (0.0, -1.0, math.inf, math.nan, 1e-40):
         with pytest.raises(ValueError, match="temperature"):
             ops.token_log_probs(logits, tokens, temperature=bad)
     if device == "cuda":
@@ -429,6 +442,8 @@ def rotate64(x, cos, sin, interleaved):
     (2, 7, 12, 4, 80, 4, 80, True, False),
     (2, 19, 5, 1, 96, 16, 48, False, False),
     (4, 5, 6, 3, 80, 1, 40, False, False),
+    (2, 9, 4, 2, 80, 16, 40, True, False),
+    (2, 9, 7, 1, 24, 16, 8, False, False),
     (2, 33, 16, 2, 256, 32, 256, True, False),
     (3, 6, 3, 3, 40, 8, 20, True, True),
     (3, 6, 2, 1, 8, 64, 8, False, True),
@@ -675,6 +690,8 @@ def test_paged_refusals(device):
         (dict(rope=(rope[0].repeat(1, 2), rope[1].repeat(1, 2))), ValueError, "rope must be"),
         (dict(rope=(rope[0][:, ::2], rope[1][:, ::2])), ValueError, "contiguous"),
         (dict(k=k.clone().requires_grad_()), ValueError, "no_grad"),
+        (dict(vc=k_cache), ValueError, "same memory"),
+        (dict(kc=k_cache[:1].expand(4, -1, -1, -1)), ValueError, "expanded"),
     ]:
         with pytest.raises(error, match=text):
             append(**bad)

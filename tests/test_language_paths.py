@@ -228,6 +228,10 @@ def test_paged_rollout_refusals():
     model = make_lm()
     with pytest.raises(ValueError, match="positions"):
         PagedGPT2Decoder(model, 2, 65, "cpu")
+    with pytest.raises(ValueError, match="vocabulary"):
+        PagedGPT2Decoder(model, 2, 20, "cpu", eos_token_id=503)
+    with pytest.raises(ValueError, match="temperature"):
+        PagedGPT2Decoder(model, 2, 20, "cpu", temperature=0.0)
     dec = PagedGPT2Decoder(model, 2, 20, "cpu", dtype=torch.float32)
     prompts = torch.zeros(2, 5, dtype=torch.long)
     with pytest.raises(ValueError, match="do not fit"):
