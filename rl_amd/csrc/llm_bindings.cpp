@@ -421,10 +421,10 @@ Tensor policy_raw(const PolicyViews& v, const PolicyConfig& c) {
 
 // The seven scalars as tensors of their own over one allocation: not views of
 // each other for autograd, so that a caller may change one in place.
-std::vector<Tensor> scalars_of(const Tensor& out) {
+std::vector<Tensor> scalars_of(const Tensor& out, int first, int last) {
   std::vector<Tensor> s;
   s.reserve(7);
-  for (int i = 0; i < 7; ++i) {
+  for (int i = first; i < last; ++i) {
     Tensor x = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(out.storage()), out.key_set(),
                                                         out.dtype());
     x.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(), at::IntArrayRef(),
@@ -434,34 +434,26 @@ std::vector<Tensor> scalars_of(const Tensor& out) {
   return s;
 }
 
+// The node of the four differentiable scalars; what they are is in `out` already.
 class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
                                                 const Tensor& log_probs, const Tensor& old_lp,
                                                 const Tensor& advantage, const OptTensor& mask,
-                                                const OptTensor& ref, int64_t variant, double low,
-                                                double high, double kl, double entropy, bool mean) {
-    const PolicyConfig c{variant, low, high, kl, entropy, mean};
-    const auto shape = log_probs.sizes();
-    PolicyViews v{matrix_of(log_probs, shape), matrix_of(old_lp, shape),
-                  matrix_of(advantage, shape), mask ? matrix_of(*mask, shape) : Tensor(),
-                  ref ? matrix_of(*ref, shape) : Tensor()};
-    Tensor out = policy_raw(v, c);
+                                                const OptTensor& ref, const Tensor& out,
+                                                const std::vector<double>& config) {
     ctx->save_for_backward({log_probs, old_lp, advantage, mask ? *mask : Tensor(),
                             ref ? *ref : Tensor(), out});
-    ctx->saved_data["config"] = std::vector<double>{(double)variant, low, high, kl, entropy,
-                                                    mean ? 1.0 : 0.0};
+    ctx->saved_data["config"] = config;
     ctx->set_materialize_grads(false);
-    auto s = scalars_of(out);
-    ctx->mark_non_differentiable({s[4], s[5], s[6]});
-    return s;
+    return scalars_of(out, 0, 4);
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "token_policy_loss: the gradient is not differentiable (create_graph)");
-    torch::autograd::variable_list none(11);
+    torch::autograd::variable_list none(7);
     if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined() && !grads[3].defined())
       return none;
     const auto saved = ctx->get_saved_variables();
@@ -504,15 +496,19 @@ std::vector<Tensor> token_policy_loss(const Tensor& log_probs, const Tensor& old
   token_policy_loss_check(log_probs, old_log_probs, advantage, mask, ref, clip_low, clip_high,
                           kl_coeff, entropy_coeff);
   TORCH_CHECK_VALUE(log_probs.is_cuda(), "token_policy_loss: expected tensors on the GPU");
-  if (at::GradMode::is_enabled() && log_probs.requires_grad())
-    return TokenPolicyLoss::apply(log_probs, old_log_probs, advantage, mask, ref, variant, clip_low,
-                                  clip_high, kl_coeff, entropy_coeff, mean);
   const auto shape = log_probs.sizes();
-  PolicyViews v{matrix_of(log_probs, shape), matrix_of(old_log_probs, shape),
-                matrix_of(advantage, shape), mask ? matrix_of(*mask, shape) : Tensor(),
-                ref ? matrix_of(*ref, shape) : Tensor()};
-  return scalars_of(
-      policy_raw(v, PolicyConfig{variant, clip_low, clip_high, kl_coeff, entropy_coeff, mean}));
+  const PolicyViews v{matrix_of(log_probs, shape), matrix_of(old_log_probs, shape),
+                      matrix_of(advantage, shape), mask ? matrix_of(*mask, shape) : Tensor(),
+                      ref ? matrix_of(*ref, shape) : Tensor()};
+  const Tensor out =
+      policy_raw(v, PolicyConfig{variant, clip_low, clip_high, kl_coeff, entropy_coeff, mean});
+  if (!(at::GradMode::is_enabled() && log_probs.requires_grad())) return scalars_of(out, 0, 7);
+  std::vector<Tensor> s = TokenPolicyLoss::apply(
+      log_probs, old_log_probs, advantage, mask, ref, out,
+      std::vector<double>{(double)variant, clip_low, clip_high, kl_coeff, entropy_coeff,
+                          mean ? 1.0 : 0.0});
+  for (Tensor& x : scalars_of(out, 4, 7)) s.push_back(std::move(x));
+  return s;
 }
 
 // ------------------------------ paged cache ------------------------------ //
