@@ -1132,10 +1132,10 @@ extern "C" long paged_attend_note_bytes(void) { return (long)sizeof(SharedItem);
 // - Workers are as many as fill the card once, no more: each has a start of its
 //   own, and shares items that must be joined.  Single waves two to a SIMD: 512
 //   items of 1 to 1024, dim 128, 41 [49 with one, 44 with three].  Workgroups one
-//   to a CU for dims above 96, whose tiles on the way (128 dim bytes to a wave)
+//   to a CU for dims from 96 on, whose tiles on the way (128 dim bytes to a wave)
 //   cover the latency, and two below: 8 items of 131072, dim 128, 101 [104 with two,
-//   113 with three]; 2 of 65536, dim 256, 40 [54]; 12 of 65536, dim 64, 45 [47 with
-//   one].
+//   113 with three]; 2 of 65536, dim 256, 40 [54]; 4 of 65536, dim 96, 26 [31]; 12 of
+//   65536, dim 64, 45 [47 with one].
 extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   const int size = a->dtype == RL_F32 ? 4 : 2;
   const int keys = size == 4 ? 16 : 32;
@@ -1152,7 +1152,7 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   }
   a->waves = items >= 256 ? 1 : 4;
   const int fit = resident_waves(a->dim, size);
-  const long fill = (long)cus * (a->waves == 1 ? 4 * (fit < 2 ? fit : 2) : a->dim > 96 ? 1 : 2);
+  const long fill = (long)cus * (a->waves == 1 ? 4 * (fit < 2 ? fit : 2) : a->dim >= 96 ? 1 : 2);
   const long worth = (items * most + a->waves - 1) / a->waves;  // a tile to each wave
   a->workers = (int)(fill < worth ? fill : worth);
 }

@@ -48,7 +48,7 @@ struct PolicyLossArgs {
   int variant;             // 0: clipped surrogate, 1: clipped weight
   double log_low, log_high;    // borders of the log ratio
   double log_off;              // upper border of the clip_fraction count
-  float low, high;             // the clipped ratio's values: 1 - low, 1 + high
+  double low, high;            // the clipped ratio's values: 1 - low, 1 + high
   double kl_coeff, entropy_coeff;
   int mean;                // 1: divide by the mask's sum, 0: plain sums
   double* partials;        // [blocks][8]
