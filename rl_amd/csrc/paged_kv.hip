@@ -1123,8 +1123,12 @@ extern "C" long paged_attend_note_bytes(void) { return (long)sizeof(SharedItem);
 // length.  Measured in us with the other choice in brackets (bf16, keys by page
 // tables of 64):
 //
-// - Short tables take one worker per item and no join: 2048 items of 16 tiles,
-//   dim 128, 100 [split: 106]; 3072 of 16, dim 64, 74 [83]; 4096 of 4 57 [65].
+// - Short tables take one worker per item and no join, whose launch costs 4: up to
+//   2048 / dim tiles, below which a single CU streams an item (some 40 GB/s) in that
+//   time.  8 items of dim 64, 500 / 800 / 1200 keys: 9.7 / 12.4 / 15.4 [split: 12.4 /
+//   13.6 / 13.5]; of dim 128, 300 / 500 / 800: 10.6 / 13.3 / 18.2 [14.5 / 13.0 / 14.9];
+//   200 items of dim 64, 800: 14 [19].  With single waves, up to 16 tiles: 2048 items
+//   of 16 tiles, dim 128, 100 [106]; 3072 of 16, dim 64, 74 [83]; 4096 of 4 57 [65].
 // - From 256 items on a worker is one wave, below a workgroup of four: ragged
 //   lengths of 1 to 1024, 768 items of dim 64, 28 [51]; 512 of dim 128 39 [64]; 1
 //   to 8192, 384 of dim 128, 160 [171]; but 16 items of 1 to 30000 38 [45], 8 of
@@ -1145,7 +1149,8 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   a->head_blocks = (group + 15) / 16;
   const long items = a->batch * a->kv_heads * a->head_blocks;
   // (a grid's y takes 65535 sequences)
-  if ((most <= 8 || (most <= 16 && items >= 1024)) && a->batch < 65536) {
+  const bool brief = most <= 8 || (items >= 1024 ? most <= 16 : most * a->dim <= 2048);
+  if (brief && a->batch < 65536) {
     a->workers = 0;
     a->waves = items >= 1024 ? 1 : 4;
     return;
