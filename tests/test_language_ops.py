@@ -90,6 +90,25 @@ def test_log_probs_and_gradient(device, dtype, shape, temperature):
         assert torch.equal(ops.token_log_probs(logits, tokens, temperature=temperature), lp)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_large_gradient(dtype):
+    """A gradient beyond 128 MB is written past the caches; some of its rows."""
+    rows, vocab = 1400, 50257
+    g = torch.Generator(device="cuda").manual_seed(0)
+    logits = torch.randn(rows, vocab, generator=g, device="cuda").mul_(3).to(dtype).requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    tokens[5] = -100
+    upstream = torch.randn(rows, generator=g, device="cuda")
+    lp = ops.token_log_probs(logits, tokens)
+    (grad,) = torch.autograd.grad(lp, logits, upstream)
+    some = [0, 1, 5, 699, 1398, 1399]
+    want, dwant, gg, p, z = log_probs_oracle(logits[some], tokens[some], 1.0, -100, upstream[some])
+    lp_tol, grad_tol = log_probs_tolerance(z, gg, p, dwant, vocab, dtype)
+    close(lp[some], want, lp_tol)
+    close(grad[some], dwant, grad_tol)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_log_probs_strided_rows(device, dtype):
@@ -593,6 +612,39 @@ def test_attend(device, dtype, lengths, heads, kv_heads, dim, page):
     close(out, want, 1.01 * half_step(want, dtype) + tol)
     again = ops.paged_attention_decode(q, k_cache, v_cache, table, count.int(), scale=dim ** -0.5)
     assert torch.equal(again, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,longest,heads,kv_heads,dim,page", [
+    (40, 700, 16, 8, 128, 16),    # single waves as workers, items shared
+    (130, 1300, 6, 3, 64, 8),     # the same, more sequences than lanes
+    (90, 1500, 20, 1, 40, 64),    # workgroups, two blocks of heads
+    (300, 120, 8, 4, 64, 16),     # one wave to an item
+    (33, 900, 24, 8, 72, 32),     # single waves, dims past the row
+])
+def test_attend_batches(dtype, batch, longest, heads, kv_heads, dim, page):
+    """Ragged batches of every way a call is split: lengths of 0, 1 and the
+    longest among them."""
+    device = "cuda"
+    g = gen(batch + dim)
+    lengths = torch.randint(0, longest + 1, (batch,), generator=g).tolist()
+    lengths[0], lengths[batch // 2], lengths[-1] = 0, longest, 1
+    k_cache, v_cache, table = make_cache(g, batch, -(-longest // page), kv_heads, page, dim, dtype, device)
+    fill_cache(g, k_cache, table, lengths)
+    fill_cache(g, v_cache, table, lengths)
+    table[1, 0] = -1
+    q = (torch.randn(batch, heads, dim, generator=g) * 2).to(dtype).to(device)
+    out = ops.paged_attention_decode(q, k_cache, v_cache, table, torch.tensor(lengths, device=device))
+    some = sorted({0, 1, 2, 63 % batch, 64 % batch, batch // 2, batch - 2, batch - 1})
+    want, tol = attend_oracle(q[some], k_cache, v_cache, table[some], [lengths[b] for b in some], dim ** -0.5)
+    close(out[some], want, 1.01 * half_step(want, dtype) + tol)
+    # the others against the same sequence by itself: a row of a batch is its own
+    alone = torch.cat([ops.paged_attention_decode(
+        q[b:b + 1], k_cache, v_cache, table[b:b + 1], torch.tensor(lengths[b:b + 1], device=device))
+        for b in range(0, batch, 7)])
+    both = (out[::7].float() - alone.float()).abs()
+    assert (both <= 2 * torch.finfo(dtype).eps * alone.float().abs() + 1e-3).all()
 
 
 @pytest.mark.parametrize("device", DEVICES)
