@@ -4,8 +4,8 @@ LLMCollector (sampling generation) → MCAdvantage (per-group whitening)
 → GRPOLoss (+ optional KL-to-reference) → Adam.
 
 Runs anywhere (CPU ok; tiny model).  For production GPT-2 decode on
-MI355X see rl_amd.modules.llm.decode.GraphedGPT2Decoder (one hipGraph
-replay per generated token — the RLHF bench's rollout engine).
+MI355X see rl_amd.modules.llm.PagedGPT2Decoder (prompts of any lengths,
+one hipGraph replay per generated token, behavior log-probs recorded).
 
 Run: python examples/grpo_llm.py [--iters 4]
 """

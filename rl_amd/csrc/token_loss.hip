@@ -11,7 +11,8 @@
 // rescaled when m grows, and leaves (m, s) for the backward pass, which reads
 // the row a second time and writes the gradient once.  z - m is taken before
 // the product with c: c m overflows for rows masked with the type's lowest
-// value.  Bound by HBM: one read forward, one read and one write backward.
+// value.  Bound by HBM: one read forward, one read and one write backward
+// (8192 x 50257 bf16: 140 us at 5.9 TB/s, 299 us at 5.5 TB/s).
 //
 // token_policy_loss.  See the section below.
 
@@ -415,7 +416,9 @@ int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
 // execution.  Dense operands take 4 tokens to an access; any other strides or
 // types go one by one through the runtime codes.  The row of a token (for an
 // advantage per row) comes from a multiplication by the column count's
-// reciprocal; 64-bit divisions took longer than the loads.
+// reciprocal; 64-bit divisions took longer than the loads.  4M tokens with all
+// terms: 19 + 4 us forward (54 MB; 2.9 TB/s in the first kernel), 16 us backward
+// (71 MB, 4.3 TB/s); 8192 tokens 10 us forward, 4 backward.
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ float operand(const PolicyOperand& o, long r, long c) {
