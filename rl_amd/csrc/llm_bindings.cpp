@@ -313,6 +313,25 @@ Tensor log_probs_raw(const Tensor& logits, const Tensor& tokens, double temperat
   return lp;
 }
 
+// The gradient (one-hot - softmax) * upstream / temperature in elementary
+// operations, for a caller who differentiates it in turn.
+Tensor log_probs_grad_plain(const Tensor& logits, const Tensor& tokens, const Tensor& upstream,
+                            double temperature, int64_t ignore_index) {
+  const Tensor gone = tokens.eq(ignore_index);
+  const Tensor known = tokens.ge(0).logical_and(tokens.lt(logits.size(-1)));
+  const Tensor g = upstream.to(torch::kFloat32).masked_fill(gone, 0);
+  Tensor x = logits.to(torch::kFloat32) / temperature;
+  // rows that pass nothing back may hold anything, and no NaN comes through them
+  const Tensor finite = x.detach().logsumexp(-1).isfinite();
+  const Tensor out = gone.logical_or(g.detach().eq(0).logical_and(finite.logical_not()));
+  x = x.masked_fill(out.unsqueeze(-1), 0);
+  const Tensor at = tokens.to(torch::kInt64).masked_fill(known.logical_not(), 0).unsqueeze(-1);
+  const Tensor hot = torch::zeros_like(x.detach()).scatter_(-1, at, 1);
+  const Tensor row = known.logical_or(gone).logical_or(g.detach().eq(0));
+  const Tensor d = (hot - x.softmax(-1)) * (g.masked_fill(row.logical_not(), NAN) / temperature).unsqueeze(-1);
+  return d.to(logits.scalar_type());
+}
+
 class TokenLogProbs : public torch::autograd::Function<TokenLogProbs> {
  public:
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
@@ -328,12 +347,15 @@ class TokenLogProbs : public torch::autograd::Function<TokenLogProbs> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(),
-                "token_log_probs: the gradient is not differentiable (create_graph)");
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &stats = saved[2];
     c10::DeviceGuard guard(logits.device());
+    if (at::GradMode::is_enabled())  // create_graph
+      return {log_probs_grad_plain(logits, saved[1], grads[0],
+                                   ctx->saved_data["temperature"].toDouble(),
+                                   ctx->saved_data["ignore_index"].toInt()),
+              Tensor(), Tensor(), Tensor()};
     const Tensor tokens = saved[1].contiguous();
     const Tensor g = grads[0].to(torch::kFloat32).contiguous();
     Tensor out = torch::empty(logits.sizes(), logits.options());
@@ -434,6 +456,33 @@ std::vector<Tensor> scalars_of(const Tensor& out, int first, int last) {
   return s;
 }
 
+// The gradient in elementary operations, in double, for a caller who
+// differentiates it in turn: by the log-probs and by the upstream gradients `g`
+// (undefined: none) of the four scalars.  `factor` is the 1 / D of the means.
+Tensor policy_grad_plain(const Tensor& log_probs, const Tensor& old_log_probs,
+                         const Tensor& advantage, const Tensor& mask, const Tensor& ref,
+                         const Tensor& factor, const PolicyConfig& c, const Tensor (&g)[4]) {
+  const auto f64 = [](const Tensor& t) { return t.to(torch::kFloat64); };
+  const auto options = log_probs.options().dtype(torch::kFloat64);
+  const Tensor w = mask.defined() ? f64(mask) : torch::ones(log_probs.sizes(), options);
+  const Tensor gone = w.eq(0);
+  const auto kept = [&](const Tensor& t) { return t.masked_fill(gone, 0); };
+  const auto up = [&](int i) { return g[i].defined() ? f64(g[i]) : torch::zeros({}, options); };
+  const Tensor total = up(0), lp = kept(f64(log_probs));
+  const Tensor adv = kept(f64(advantage).expand(log_probs.sizes()));
+  const Tensor x = kept(lp - f64(old_log_probs)), ratio = x.exp();
+  const Tensor above = x.detach().gt(std::log1p(c.high));
+  const Tensor below = c.low < 1 ? x.detach().lt(std::log1p(-c.low)) : torch::zeros_like(above);
+  const Tensor against = above.logical_and(adv.gt(0)).logical_or(below.logical_and(adv.lt(0)));
+  const Tensor dgain =
+      adv * (c.variant == 0
+                 ? ratio.masked_fill(against, 0)
+                 : ratio.detach().masked_fill(above, 1 + c.high).masked_fill(below, 1 - c.low));
+  Tensor d = (total + up(3)) * c.entropy - (total + up(1)) * dgain;
+  if (ref.defined()) d = d - (total + up(2)) * c.kl * kept(f64(ref) - lp).expm1();
+  return kept(d * w * f64(factor)).to(log_probs.scalar_type());
+}
+
 // The node of the four differentiable scalars; what they are is in `out` already.
 class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
  public:
@@ -451,14 +500,19 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(),
-                "token_policy_loss: the gradient is not differentiable (create_graph)");
     torch::autograd::variable_list none(7);
     if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined() && !grads[3].defined())
       return none;
     const auto saved = ctx->get_saved_variables();
     const auto cfg = ctx->saved_data["config"].toDoubleVector();
     const PolicyConfig c{(int64_t)cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5] != 0.0};
+    if (at::GradMode::is_enabled()) {  // create_graph
+      c10::DeviceGuard guard(saved[0].device());
+      none[0] = policy_grad_plain(saved[0], saved[1], saved[2], saved[3], saved[4],
+                                  saved[5].select(0, 7), c,
+                                  {grads[0], grads[1], grads[2], grads[3]});
+      return none;
+    }
     const auto shape = saved[0].sizes();
     PolicyViews v;
     v.log_probs = matrix_of(saved[0], shape);

@@ -63,8 +63,9 @@ def token_log_probs(
         temperature: positive (1e-30 to 1e30).
 
     Returns:
-        ``[...]`` float32.  Differentiable in ``logits`` (once); the gradient
-        has the logits' dtype.  A place with an upstream gradient of 0 gets a
+        ``[...]`` float32.  Differentiable in ``logits``; the gradient has
+        the logits' dtype, and is itself differentiable in elementary operations
+        (``create_graph``).  A place with an upstream gradient of 0 gets a
         gradient of exactly 0 whatever its logits hold.  A row of nothing but
         ``-inf`` gives NaN.
     """

@@ -241,9 +241,40 @@ def test_log_probs_refusals(device):
     if device == "cuda":
         with pytest.raises(ValueError, match="tokens is on"):
             ops.token_log_probs(logits, tokens.cpu())
-        leaf = logits.clone().requires_grad_()
-        with pytest.raises(RuntimeError, match="create_graph"):
-            torch.autograd.grad(ops.token_log_probs(leaf, tokens).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_log_probs_second_derivative(device):
+    """A product of the Hessian with a vector, and the gradient's derivative by
+    the upstream one, an ignored place, a NaN row without upstream among them."""
+    g = gen(12)
+    logits = torch.randn(5, 37, generator=g) * 2
+    tokens = torch.randint(0, 37, (5,), generator=g)
+    tokens[1] = -100
+    upstream, vec = torch.randn(5, generator=g), torch.randn(5, 37, generator=g)
+
+    def products(x, up, at, v, call):
+        x, up = x.requires_grad_(), up.requires_grad_()
+        (first,) = torch.autograd.grad(call(x, at), x, up, create_graph=True)
+        return (first, *torch.autograd.grad((first * v).sum(), (x, up)))
+
+    def plain(x, at):
+        lp = (x / 1.7).log_softmax(-1).gather(-1, at.clamp(min=0)[:, None]).squeeze(-1)
+        return torch.where(at == -100, 0.0, lp)
+
+    got = products(logits.to(device), upstream.to(device), tokens.to(device), vec.to(device),
+                   lambda x, at: ops.token_log_probs(x, at, temperature=1.7))
+    want = products(logits.double(), upstream.double(), tokens, vec.double(), plain)
+    for a, b in zip(got, want):
+        # sums over 37 products of terms up to 5, some 100 roundings
+        assert (a.detach().cpu().double() - b.detach()).abs().max() <= 100 * U * 5 * 5
+    if device == "cuda":
+        x = logits.cuda()
+        x[3] = math.nan
+        up = upstream.cuda()
+        up[3] = 0
+        first = products(x, up, tokens.cuda(), vec.cuda(), lambda x, at: ops.token_log_probs(x, at))[0]
+        assert (first[3] == 0).all() and (first[1] == 0).all() and first.isfinite().all()
 
 
 # --------------------------------------------------------------------------- #
@@ -425,10 +456,51 @@ def test_policy_loss_refusals(device):
         call(variant="ppo")
     with pytest.raises(ValueError, match="reduction"):
         call(reduction="none")
-    if device == "cuda":
-        leaf = lp.clone().requires_grad_()
-        with pytest.raises(RuntimeError, match="create_graph"):
-            torch.autograd.grad(call(a=leaf).loss_total, leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("variant", ["clip", "cispo"])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_policy_loss_second_derivative(device, variant, reduction):
+    """The gradient's derivative by the log-probs and by the upstream gradients
+    of all four scalars; a masked place holds NaN."""
+    g = gen(13)
+    old = -torch.rand(4, 9, generator=g) * 2
+    lp = old + 0.3 * torch.randn(4, 9, generator=g)
+    adv, ref = torch.randn(4, 1, generator=g), old + 0.2 * torch.randn(4, 9, generator=g)
+    mask = torch.rand(4, 9, generator=g) < 0.8
+    mask[0, 0] = False
+    vec = torch.randn(4, 9, generator=g)
+    conf = dict(clip_high=0.28, kl_coeff=0.3, entropy_coeff=0.1)
+
+    def products(scalars, lp, v):
+        ups = [torch.tensor(u, dtype=lp.dtype, device=lp.device, requires_grad=True)
+               for u in (0.7, -1.1, 0.4, 2.0)]
+        (first,) = torch.autograd.grad(scalars, lp, ups, create_graph=True)
+        first = torch.where(mask.to(lp.device), first, 0)
+        return (first, *torch.autograd.grad((first * v).sum(), (lp, *ups)))
+
+    x = lp.clone()
+    x[0, 0] = math.nan
+    x = x.to(device).requires_grad_()
+    out = ops.token_policy_loss(x, old.to(device), adv.to(device), mask.to(device), ref.to(device),
+                                variant=variant, reduction=reduction, **conf)
+    got = products(out[:4], x, vec.to(device))
+
+    y = lp.double().requires_grad_()
+    w = mask.double()
+    r = (y - old.double()).exp()
+    c = r.clamp(0.8, 1.28)
+    a = adv.double()
+    gain = torch.minimum(r * a, c * a) if variant == "clip" else c.detach() * (y - old.double()) * a
+    n = w.sum() if reduction == "mean" else 1.0
+    d = ref.double() - y
+    obj, kl, ent = -(gain * w).sum() / n, 0.3 * ((d.exp() - 1 - d) * w).sum() / n, 0.1 * (y * w).sum() / n
+    want = products((obj + kl + ent, obj, kl, ent), y, vec.double())
+    for a, b in zip(got, want):
+        # terms up to some 20, 36 of them in a sum, 40 roundings each
+        size = 20 * (1 if reduction == "mean" else 36)
+        assert (a.detach().cpu().double() - b.detach()).abs().max() <= 40 * U * size
 
 
 # --------------------------------------------------------------------------- #
