@@ -121,20 +121,31 @@ class GRPOLoss(LossModule):
             kl_coeff=self.kl_to_ref_coeff if ref_lp is not None else 0.0,
             entropy_coeff=self.entropy_coeff or 0.0,
             reduction="mean" if self.reduction == "mean" else "sum")
-        dtype = new_lp.dtype
+
+        # the types that the plain form's operations give: those of a 0-dim operand
+        # and of integer masks do not count; autocast takes exp and sum to float32
+        def typed(value, *operands):
+            dtype = new_lp.dtype
+            if torch.is_autocast_enabled("cuda"):
+                dtype = torch.float32
+            for t in operands:
+                if t is not None and t.is_floating_point() and (t.dim() or not new_lp.dim()):
+                    dtype = torch.promote_types(dtype, t.dtype)
+            return value.to(dtype)
+
         out = TensorDict(
             {
-                "loss_objective": loss.loss_objective.to(dtype),
+                "loss_objective": typed(loss.loss_objective, old_lp, adv, mask),
                 "clip_fraction": loss.clip_fraction,
-                "ESS": loss.ess.to(dtype),
+                "ESS": typed(loss.ess, old_lp),
             },
             batch_size=[],
         )
         if ref_lp is not None:
-            out.set("loss_kl_to_ref", loss.loss_kl.to(dtype))
-            out.set("kl_to_ref", loss.kl.to(dtype))
+            out.set("loss_kl_to_ref", typed(loss.loss_kl, ref_lp, mask))
+            out.set("kl_to_ref", typed(loss.kl, ref_lp, mask))
         if self.entropy_coeff:
-            out.set("loss_entropy", loss.loss_entropy.to(dtype))
+            out.set("loss_entropy", typed(loss.loss_entropy, mask))
         return out
 
     def forward(self, tensordict: TensorDictBase) -> TensorDictBase:
