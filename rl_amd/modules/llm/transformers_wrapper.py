@@ -13,6 +13,7 @@ from typing import Any, List, Optional, Sequence, Union
 import torch
 
 from ... import ops
+from ...ops.language import _ordinary
 from ...data.llm.history import History
 from ...tensordict import NonTensorData, TensorDict, TensorDictBase, TensorDictModuleBase
 
@@ -22,7 +23,11 @@ __all__ = ["LLMWrapperBase", "TransformersWrapper"]
 def _log_probs_of(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     """``log_softmax(logits)`` at ``tokens``, in the logits' dtype (float32 under
     autocast, as ``log_softmax`` itself)."""
-    if logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
+    if (
+        logits.is_cuda
+        and logits.dtype in (torch.float32, torch.bfloat16, torch.float16)
+        and _ordinary(logits, tokens)
+    ):
         lp = ops.token_log_probs(logits, tokens)
         return lp if torch.is_autocast_enabled("cuda") else lp.to(logits.dtype)
     return logits.log_softmax(-1).gather(-1, tokens.unsqueeze(-1)).squeeze(-1)

@@ -11,6 +11,7 @@ from typing import Optional
 import torch
 
 from ... import ops
+from ...ops.language import _ordinary
 from ...tensordict import TensorDict, TensorDictBase, TensorDictModuleBase
 from ..common import LossModule
 
@@ -95,12 +96,14 @@ class GRPOLoss(LossModule):
     def _fused(self, new_lp, old_lp, adv, mask, ref_lp) -> Optional[TensorDictBase]:
         """The losses from one kernel, or None where it does not apply: off
         the GPU, for a subclass with a gain or reduction of its own, for
-        operands that broadcast or carry gradients themselves."""
+        operands that broadcast or carry gradients themselves, under
+        function transforms."""
         owner = next(c for c in type(self).__mro__ if "_ratio_clip_gain" in c.__dict__)
         data = [t for t in (old_lp, adv, mask, ref_lp) if t is not None]
         same = [t for t in (old_lp, mask, ref_lp) if t is not None]
         if (
             not new_lp.is_cuda
+            or not _ordinary(new_lp, *data)
             or "_fused_clip" not in owner.__dict__
             or type(self)._reduce is not GRPOLoss._reduce
             or new_lp.numel() == 0

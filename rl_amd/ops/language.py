@@ -40,6 +40,18 @@ def _native(tensor: torch.Tensor):
     return _C if tensor.is_cuda and _require_ext() else None
 
 
+def _ordinary(*tensors: torch.Tensor) -> bool:
+    """Whether all are tensors whose memory a kernel can take: not subclasses,
+    not under functorch's transforms, forward derivatives or a tracing compiler.
+    What offers an operator in place of elementary torch asks this first."""
+    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level >= 0:
+        return False
+    return all(
+        type(t) in (torch.Tensor, torch.nn.Parameter)
+        and not torch._C._functorch.is_functorch_wrapped_tensor(t)
+        for t in tensors)
+
+
 # --------------------------------------------------------------------------- #
 # token log-probabilities
 # --------------------------------------------------------------------------- #

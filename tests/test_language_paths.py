@@ -444,6 +444,46 @@ def test_wrapper_log_probs_under_autocast():
     assert (got - want).abs().max() <= 64 * U * 10
 
 
+class Wrapped(torch.Tensor):
+    """A subclass that sees every operation on it, as sharded tensors do."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+@pytest.mark.gpu
+def test_transforms_and_subclasses_keep_the_plain_form():
+    """vmap, forward and functional derivatives and tensor subclasses go through
+    the losses and wrappers as they did."""
+    from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
+
+    g = torch.Generator().manual_seed(7)
+    lp, old, adv = torch.randn(3, 2, 5, generator=g).cuda()
+    td = TensorDict({"log_probs": old, "advantage": adv}, batch_size=[2])
+
+    def loss(x):
+        return GRPOLoss(Given(x))(td).get("loss_objective")
+
+    leaf = lp.clone().requires_grad_()
+    (want,) = torch.autograd.grad(loss(leaf), leaf)
+    assert torch.allclose(torch.func.grad(loss)(lp), want, atol=1e-6)
+    many = torch.func.vmap(loss)(torch.stack([lp, lp + 0.1]))
+    assert torch.allclose(many, torch.stack([loss(lp), loss(lp + 0.1)]), atol=1e-6)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(lp, torch.ones_like(lp))
+        tangent = torch.autograd.forward_ad.unpack_dual(loss(dual)).tangent
+    assert torch.allclose(tangent, want.sum(), atol=1e-6)
+    assert torch.allclose(loss(lp.as_subclass(Wrapped)), loss(lp), atol=1e-6)
+    assert type(loss(lp.as_subclass(Wrapped))) is Wrapped
+
+    logits = torch.randn(2, 5, 11, generator=g).cuda()
+    tokens = torch.randint(0, 11, (2, 5), generator=g).cuda()
+    rows = torch.func.vmap(_log_probs_of)(logits, tokens)
+    assert torch.allclose(rows, _log_probs_of(logits, tokens), atol=1e-5)
+    assert type(_log_probs_of(logits.as_subclass(Wrapped), tokens)) is Wrapped
+
+
 # --------------------------------------------------------------------------- #
 # streams, graphs, far offsets
 # --------------------------------------------------------------------------- #
