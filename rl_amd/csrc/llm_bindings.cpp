@@ -10,6 +10,7 @@
 
 #include <ATen/core/grad_mode.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -424,12 +425,12 @@ PolicyLossArgs policy_args(const PolicyViews& v, const PolicyConfig& c) {
   return a;
 }
 
-// The seven scalars and the factor that the backward pass needs, in one buffer.
+// The seven scalars and the three numbers that the backward pass needs, in one buffer.
 Tensor policy_raw(const PolicyViews& v, const PolicyConfig& c) {
   c10::DeviceGuard guard(v.log_probs.device());
   PolicyLossArgs a = policy_args(v, c);
   a.blocks = policy_loss_blocks(a.rows * a.cols);
-  Tensor out = torch::empty({8}, v.log_probs.options().dtype(torch::kFloat32));
+  Tensor out = torch::empty({10}, v.log_probs.options().dtype(torch::kFloat32));
   Tensor partials;
   if (a.blocks > 1) {
     partials = torch::empty({a.blocks, 8}, v.log_probs.options().dtype(torch::kFloat64));
@@ -458,10 +459,10 @@ std::vector<Tensor> scalars_of(const Tensor& out, int first, int last) {
 
 // The gradient in elementary operations, in double, for a caller who
 // differentiates it in turn: by the log-probs and by the upstream gradients `g`
-// (undefined: none) of the four scalars.  `factor` is the 1 / D of the means.
+// (undefined: none) of the five scalars.  `factor` is the 1 / D of the means.
 Tensor policy_grad_plain(const Tensor& log_probs, const Tensor& old_log_probs,
                          const Tensor& advantage, const Tensor& mask, const Tensor& ref,
-                         const Tensor& factor, const PolicyConfig& c, const Tensor (&g)[4]) {
+                         const Tensor& factor, const PolicyConfig& c, const Tensor (&g)[5]) {
   const auto f64 = [](const Tensor& t) { return t.to(torch::kFloat64); };
   const auto options = log_probs.options().dtype(torch::kFloat64);
   const Tensor w = mask.defined() ? f64(mask) : torch::ones(log_probs.sizes(), options);
@@ -480,10 +481,18 @@ Tensor policy_grad_plain(const Tensor& log_probs, const Tensor& old_log_probs,
                  : ratio.detach().masked_fill(above, 1 + c.high).masked_fill(below, 1 - c.low));
   Tensor d = (total + up(3)) * c.entropy - (total + up(1)) * dgain;
   if (ref.defined()) d = d - (total + up(2)) * c.kl * kept(f64(ref) - lp).expm1();
-  return kept(d * w * f64(factor)).to(log_probs.scalar_type());
+  d = kept(d * w * f64(factor));
+  if (g[4].defined()) {
+    const Tensor r = (f64(log_probs) - f64(old_log_probs)).exp();
+    const Tensor squares = r.square().sum();
+    const Tensor t = r * (r.sum() / squares.clamp_min(1e-9));
+    const Tensor live = squares.detach().ge(1e-9).to(torch::kFloat64);
+    d = d + up(4) * (2.0 / (double)log_probs.numel()) * (t - live * t.square());
+  }
+  return d.to(log_probs.scalar_type());
 }
 
-// The node of the four differentiable scalars; what they are is in `out` already.
+// The node of the five differentiable scalars; what they are is in `out` already.
 class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
@@ -495,13 +504,15 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
                             ref ? *ref : Tensor(), out});
     ctx->saved_data["config"] = config;
     ctx->set_materialize_grads(false);
-    return scalars_of(out, 0, 4);
+    std::vector<Tensor> s = scalars_of(out, 0, 4);
+    for (Tensor& x : scalars_of(out, 6, 7)) s.push_back(std::move(x));
+    return s;
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     torch::autograd::variable_list none(7);
-    if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined() && !grads[3].defined())
+    if (std::none_of(grads.begin(), grads.end(), [](const Tensor& g) { return g.defined(); }))
       return none;
     const auto saved = ctx->get_saved_variables();
     const auto cfg = ctx->saved_data["config"].toDoubleVector();
@@ -510,7 +521,7 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
       c10::DeviceGuard guard(saved[0].device());
       none[0] = policy_grad_plain(saved[0], saved[1], saved[2], saved[3], saved[4],
                                   saved[5].select(0, 7), c,
-                                  {grads[0], grads[1], grads[2], grads[3]});
+                                  {grads[0], grads[1], grads[2], grads[3], grads[4]});
       return none;
     }
     const auto shape = saved[0].sizes();
@@ -523,9 +534,9 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
     c10::DeviceGuard guard(saved[0].device());
     PolicyLossArgs a = policy_args(v, c);
     a.scale = saved[5].data_ptr<float>() + 7;
-    Tensor g[4];
-    const float* p[4] = {};
-    for (int i = 0; i < 4; ++i)
+    Tensor g[5];
+    const float* p[5] = {};
+    for (int i = 0; i < 5; ++i)
       if (grads[i].defined()) {
         g[i] = grads[i].to(torch::kFloat32);
         p[i] = g[i].data_ptr<float>();
@@ -534,6 +545,7 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
     a.g_objective = p[1];
     a.g_kl = p[2];
     a.g_entropy = p[3];
+    a.g_ess = p[4];
     Tensor out = torch::empty(shape, saved[0].options());
     a.grad = out.data_ptr();
     launched(launch_policy_loss_bwd(&a, stream_of()), "token_policy_loss");
@@ -561,7 +573,8 @@ std::vector<Tensor> token_policy_loss(const Tensor& log_probs, const Tensor& old
       log_probs, old_log_probs, advantage, mask, ref, out,
       std::vector<double>{(double)variant, clip_low, clip_high, kl_coeff, entropy_coeff,
                           mean ? 1.0 : 0.0});
-  for (Tensor& x : scalars_of(out, 4, 7)) s.push_back(std::move(x));
+  std::vector<Tensor> data = scalars_of(out, 4, 6);
+  s.insert(s.begin() + 4, data.begin(), data.end());
   return s;
 }
 

@@ -54,12 +54,14 @@ struct PolicyLossArgs {
   double* partials;        // [blocks][8]
   int blocks;
   float* out;              // 7 scalars
-  float* scale;            // 1 / denominator, for the backward pass
+  float* scale;            // for the backward pass: 1 / denominator; log2 of the ess'
+                           // sum(r) / sum(r^2); whether sum(r^2) is above its floor
   // backward
   const float* g_total;    // upstream scalars; null: zero
   const float* g_objective;
   const float* g_kl;
   const float* g_entropy;
+  const float* g_ess;
   void* grad;              // [rows][cols] dense, log_probs' type
 };
 

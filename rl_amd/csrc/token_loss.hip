@@ -402,6 +402,8 @@ int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
 //   kl:     e^y - 1 - y with y = ref - lp;  d/dlp = 1 - e^y
 //   entropy term: + lp (the sampled estimate of -H); d/dlp = 1
 //   objective = -sum w gain / D, and the rest likewise
+//   ess = S^2 / (Q n) over all n places, S = sum r, Q = sum r^2;
+//           dess/dlp = 2 / n (t - t^2) with t = r S / Q
 //
 // Whether a ratio is clipped is decided in double on x against the borders'
 // logarithms, so that an element next to a border is treated as in the definition.
@@ -497,22 +499,31 @@ __device__ __forceinline__ void policy_terms(const PolicyLossArgs& a, float lp, 
   if (has_ref) s[S_KL] += (double)w * kl3(ref - lp);
 }
 
-// What a token's gradient is, before its upstream factors are folded in:
-// go, gk and ge carry the upstream gradients, coefficients and 1 / D.
+// The upstream gradients with their coefficients and 1 / D, or 2 / n.
+struct PolicyUpstream {
+  float go, gk, ge;
+  float ess, ess_log2, ess_live;
+};
+
 __device__ __forceinline__ float policy_grad(const PolicyLossArgs& a, float lp, float old, float adv,
-                                             float w, float ref, bool has_ref, float go, float gk,
-                                             float ge) {
-  if (w == 0.f) return 0.f;
+                                             float w, float ref, bool has_ref,
+                                             const PolicyUpstream& u) {
+  float e = 0.f;
+  if (u.ess != 0.f) {  // of masked tokens too
+    const float t = exp2_hw(fmaf((float)((double)lp - (double)old), kLog2e, u.ess_log2));
+    e = u.ess * (t - u.ess_live * t * t);
+  }
+  if (w == 0.f) return e;
   const PolicyToken t = policy_token(a, lp, old);
   const float ratio = exp2_hw((float)t.x * kLog2e);
   const float dgain = a.variant == 0 ? (clipped_against(t, adv) ? 0.f : ratio * adv)
                                      : (t.above ? (float)a.high : t.below ? (float)a.low : ratio) * adv;
-  float d = ge - go * dgain;
+  float d = u.ge - u.go * dgain;
   if (has_ref) {
     const float y = ref - lp;
-    d -= gk * (kl3(y) + y);
+    d -= u.gk * (kl3(y) + y);
   }
-  return d * w;
+  return fmaf(d, w, e);
 }
 
 __device__ __forceinline__ void policy_finish(const PolicyLossArgs& a, const double (&s)[S_COUNT]) {
@@ -528,7 +539,9 @@ __device__ __forceinline__ void policy_finish(const PolicyLossArgs& a, const dou
   a.out[4] = (float)kl;
   a.out[5] = (float)(s[S_OFF] / n);
   a.out[6] = (float)(s[S_R] * s[S_R] / fmax(s[S_RR], 1e-9) / n);
-  *a.scale = (float)inv;
+  a.scale[0] = (float)inv;
+  a.scale[1] = (float)log2(s[S_R] / fmax(s[S_RR], 1e-9));
+  a.scale[2] = s[S_RR] >= 1e-9 ? 1.f : 0.f;
 }
 
 template <int BLOCK>
@@ -663,16 +676,14 @@ __global__ __launch_bounds__(512) void policy_loss_join_k(const PolicyLossArgs a
   if (block_sums<512>(s)) policy_finish(a, s);
 }
 
-struct PolicyUpstream {
-  float go, gk, ge;
-};
-
 __device__ __forceinline__ PolicyUpstream policy_upstream(const PolicyLossArgs& a) {
   const float inv = *a.scale;
   const float total = a.g_total ? *a.g_total : 0.f;
   return {(total + (a.g_objective ? *a.g_objective : 0.f)) * inv,
           (float)((total + (a.g_kl ? *a.g_kl : 0.f)) * a.kl_coeff * inv),
-          (float)((total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv)};
+          (float)((total + (a.g_entropy ? *a.g_entropy : 0.f)) * a.entropy_coeff * inv),
+          (a.g_ess ? *a.g_ess : 0.f) * (float)(2.0 / ((double)a.rows * (double)a.cols)), a.scale[1],
+          a.scale[2]};
 }
 
 template <typename T>
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(256) void policy_loss_dense_bwd_k(const PolicyLossA
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       q.x[k] = (T)policy_grad(a, f.lp[k], f.old[k], f.adv[k], f.w[k], has_ref ? f.ref[k] : 0.f, has_ref,
-                              u.go, u.gk, u.ge);
+                              u);
     if (i + 4 <= n) {
       *(Q*)((T*)a.grad + i) = q;
     } else {
@@ -710,7 +721,7 @@ __global__ __launch_bounds__(256) void policy_loss_bwd_k(const PolicyLossArgs a)
     const long r = n < (1L << 31) ? row_of(a, (unsigned)i) : i / a.cols, c = i - r * a.cols;
     ((T*)a.grad)[i] = (T)policy_grad(a, operand(a.log_probs, r, c), operand(a.old_log_probs, r, c),
                                      operand(a.advantage, r, c), a.mask.ptr ? operand(a.mask, r, c) : 1.f,
-                                     has_ref ? operand(a.ref, r, c) : 0.f, has_ref, u.go, u.gk, u.ge);
+                                     has_ref ? operand(a.ref, r, c) : 0.f, has_ref, u);
   }
 }
 

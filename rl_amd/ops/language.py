@@ -101,7 +101,7 @@ def token_log_probs(
 # --------------------------------------------------------------------------- #
 class TokenPolicyLoss(NamedTuple):
     """What :func:`token_policy_loss` returns: float32 scalars.  The first
-    four carry a gradient to ``log_probs``."""
+    four and ``ess`` carry a gradient to ``log_probs``."""
 
     loss_total: torch.Tensor
     loss_objective: torch.Tensor
@@ -149,8 +149,8 @@ def token_policy_loss(
             others must not require one.
         advantage: broadcasts to ``log_probs``.
         mask: bool, integer or float weights of ``log_probs``' shape.  A place
-            of weight 0 may hold anything (its gradient is 0), though what it
-            holds still enters ``clip_fraction`` and ``ess``.
+            of weight 0 may hold anything (the losses' gradient there is 0),
+            though what it holds still enters ``clip_fraction`` and ``ess``.
         reduction: ``"mean"`` as above, or ``"sum"``: the weighted sums, not
             divided.
     """
@@ -170,8 +170,7 @@ def token_policy_loss(
     lp, old = log_probs.float(), old_log_probs.float()
     w = torch.ones_like(lp) if mask is None else mask.float()
     gone = w == 0
-    with torch.no_grad():
-        every = (lp - old).exp()
+    every = (lp - old).exp()
     # masked places are replaced before anything is computed of them: a NaN
     # there would come back through the backward pass as 0 * NaN
     lp = torch.where(gone, 0.0, lp)
@@ -187,9 +186,8 @@ def token_policy_loss(
         y = torch.where(gone, 0.0, ref_log_probs.float() - lp)
         kl = ((torch.expm1(y) - y) * w).sum() / count
     entropy = entropy_coeff * (lp * w).sum() / count
-    with torch.no_grad():
-        off = ((every - 1).abs() > clip_low).float().mean()
-        ess = every.sum().square() / every.square().sum().clamp(min=1e-9) / every.numel()
+    off = ((every.detach() - 1).abs() > clip_low).float().mean()
+    ess = every.sum().square() / every.square().sum().clamp(min=1e-9) / every.numel()
     return TokenPolicyLoss(
         objective + kl_coeff * kl + entropy, objective, kl_coeff * kl, entropy, kl.detach(), off, ess)
 

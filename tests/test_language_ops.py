@@ -459,11 +459,50 @@ def test_policy_loss_refusals(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,shift", [((1, 1), 0.0), ((5, 33), 0.0), ((5, 33), 60.0), ((5, 33), -12.0),
+                                         ((130, 257), 0.0)])
+@pytest.mark.parametrize("dense", [False, True])
+def test_policy_loss_ess_gradient(device, dtype, shape, shift, dense):
+    """Alone and with the loss's, masked places among them; ratios so large that
+    their squares leave float32, and so small that the sum meets its floor."""
+    g = gen(14)
+    old = (-torch.rand(shape, generator=g) * 2).to(dtype)
+    lp = (old.float() + shift + 0.4 * torch.randn(shape, generator=g)).to(dtype)
+    adv = torch.randn(shape, generator=g)
+    mask = torch.rand(shape, generator=g) < 0.6
+    x = lp.to(device)
+    if not dense:
+        x = x.t().contiguous().t()
+    x.requires_grad_()
+    out = ops.token_policy_loss(x, old.to(device), adv.to(device), mask.to(device))
+    y = lp.double().requires_grad_()
+    r = (y - old.double()).exp()
+    ess = r.sum() ** 2 / (r ** 2).sum().clamp(min=1e-9) / r.numel()
+    (want,) = torch.autograd.grad(ess, y)
+    if device == "cpu" and shift == 60.0:
+        return  # elementary float32 overflows here
+    (got,) = torch.autograd.grad(1.5 * out.ess, x, retain_graph=True)
+    t = (r * r.sum() / (r ** 2).sum().clamp(min=1e-9)).detach()
+    size = 1.5 * 2 / r.numel() * (t + t * t)
+    # the exponent's argument is off by u of its size, up to some 100 in base 2;
+    # float32 sums on the CPU add their length's root
+    tol = size * U * 400 * (4 if device == "cpu" else 1) + 1.5 * want.abs() * torch.finfo(dtype).eps / 2 + 1e-30
+    tiny = torch.finfo(dtype).smallest_normal
+    assert ((got.cpu().double() - 1.5 * want).abs() <= tol + tiny).all()
+    if shift == 0.0:
+        (both,) = torch.autograd.grad(1.5 * out.ess + out.loss_total, x, retain_graph=True)
+        (loss,) = torch.autograd.grad(out.loss_total, x)
+        assert ((both - got - loss).abs().double().cpu()
+                <= 3 * torch.finfo(dtype).eps * (got.abs() + loss.abs()).double().cpu() + tiny).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("variant", ["clip", "cispo"])
 @pytest.mark.parametrize("reduction", ["mean", "sum"])
 def test_policy_loss_second_derivative(device, variant, reduction):
     """The gradient's derivative by the log-probs and by the upstream gradients
-    of all four scalars; a masked place holds NaN."""
+    of all five scalars; a masked place is far off."""
     g = gen(13)
     old = -torch.rand(4, 9, generator=g) * 2
     lp = old + 0.3 * torch.randn(4, 9, generator=g)
@@ -474,18 +513,17 @@ def test_policy_loss_second_derivative(device, variant, reduction):
     conf = dict(clip_high=0.28, kl_coeff=0.3, entropy_coeff=0.1)
 
     def products(scalars, lp, v):
+        assert len(scalars) == 5
         ups = [torch.tensor(u, dtype=lp.dtype, device=lp.device, requires_grad=True)
-               for u in (0.7, -1.1, 0.4, 2.0)]
+               for u in (0.7, -1.1, 0.4, 2.0, 1.3)]
         (first,) = torch.autograd.grad(scalars, lp, ups, create_graph=True)
-        first = torch.where(mask.to(lp.device), first, 0)
         return (first, *torch.autograd.grad((first * v).sum(), (lp, *ups)))
 
-    x = lp.clone()
-    x[0, 0] = math.nan
-    x = x.to(device).requires_grad_()
+    lp[0, 0] = old[0, 0] - 9.0
+    x = lp.to(device).requires_grad_()
     out = ops.token_policy_loss(x, old.to(device), adv.to(device), mask.to(device), ref.to(device),
                                 variant=variant, reduction=reduction, **conf)
-    got = products(out[:4], x, vec.to(device))
+    got = products((*out[:4], out.ess), x, vec.to(device))
 
     y = lp.double().requires_grad_()
     w = mask.double()
@@ -496,11 +534,21 @@ def test_policy_loss_second_derivative(device, variant, reduction):
     n = w.sum() if reduction == "mean" else 1.0
     d = ref.double() - y
     obj, kl, ent = -(gain * w).sum() / n, 0.3 * ((d.exp() - 1 - d) * w).sum() / n, 0.1 * (y * w).sum() / n
-    want = products((obj + kl + ent, obj, kl, ent), y, vec.double())
+    ess = r.sum() ** 2 / (r ** 2).sum() / r.numel()
+    want = products((obj + kl + ent, obj, kl, ent, ess), y, vec.double())
     for a, b in zip(got, want):
-        # terms up to some 20, 36 of them in a sum, 40 roundings each
+        # terms up to some 20 (e^9 of the masked one has weight 0), 36 of them in a
+        # sum, 40 roundings each
         size = 20 * (1 if reduction == "mean" else 36)
         assert (a.detach().cpu().double() - b.detach()).abs().max() <= 40 * U * size
+
+    x = lp.clone()
+    x[0, 0] = math.nan  # masked: nothing of it comes back without the ess
+    x = x.to(device).requires_grad_()
+    total = ops.token_policy_loss(x, old.to(device), adv.to(device), mask.to(device), ref.to(device),
+                                  variant=variant, reduction=reduction, **conf).loss_total
+    (first,) = torch.autograd.grad(total, x, create_graph=True)
+    assert first.isfinite().all() and first[0, 0] == 0
 
 
 # --------------------------------------------------------------------------- #

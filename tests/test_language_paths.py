@@ -361,7 +361,8 @@ def test_grpo_family_on_the_gpu_equals_the_plain_form(loss_cls, reduction, with_
         loss = loss_cls(Given(lp), kl_to_ref_coeff=0.1, entropy_coeff=0.02, reduction=reduction)
         vals = loss(TensorDict({k: v.to(device) if not v.is_floating_point() else v.to(device, dtype)
                                 for k, v in data.items()}, batch_size=[6]))
-        (grad,) = torch.autograd.grad(sum(vals.get(k) for k in vals.keys() if k.startswith("loss")), lp)
+        (grad,) = torch.autograd.grad(
+            sum(vals.get(k) for k in vals.keys() if k.startswith("loss")) + 0.5 * vals.get("ESS"), lp)
         return {k: vals.get(k).detach().cpu().double() for k in vals.keys()}, grad.cpu().double(), vals
 
     got, grad, vals = run("cuda", torch.float32)
