@@ -419,7 +419,7 @@ int log_probs_any(const TokenLogProbArgs* a, bool bwd, void* stream) {
 // types go one by one through the runtime codes.  The row of a token (for an
 // advantage per row) comes from a multiplication by the column count's
 // reciprocal; 64-bit divisions took longer than the loads.  4M tokens with all
-// terms: 19 + 4 us forward (54 MB; 2.9 TB/s in the first kernel), 16 us backward
+// terms: 19 + 4 us forward (54 MB; 2.9 TB/s in the first kernel), 17 us backward
 // (71 MB, 4.3 TB/s); 8192 tokens 10 us forward, 4 backward.
 // ---------------------------------------------------------------------------
 
