@@ -207,8 +207,12 @@ int append_vec(const PagedAppendArgs& a, hipStream_t st) {
 // and a tile of keys costs two shuffles.  Weights enter the second product as
 // two 16-bit parts (the rounded weight and what it left), so that they are not
 // rounded to 8 bits for bfloat16; the matrix unit has the time, the kernel is
-// bound by the cache's bytes.  float32 caches use the fp32 matrix instruction on
-// tiles of 16 keys, with V's operand read directly.
+// bound by the cache's bytes.  Halves end at 2^-24, where weights relative to the
+// maximum would be cut off from 17 nats below it on and yet count in the sum, so
+// float16 weights are all taken times 2^15, in sum, output and parts alike: each is
+// right to 2^-22 of itself or 2^-40 of the largest weight, whichever is more
+// (bfloat16, with float32's exponents: 2^-17 of itself).  float32 caches use the fp32
+// matrix instruction on tiles of 16 keys, with V's operand read directly.
 //
 // A wave owns whole tiles: while it computes one, the keys and values of the next
 // are on their way in its registers, and the page ids of the one after.  No barrier
@@ -238,6 +242,7 @@ struct Matrix;
 template <>
 struct Matrix<__bf16> {
   typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+  static constexpr float WEIGHT = 1.f;
   static __device__ __forceinline__ f32x4 mul(V8 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -246,6 +251,7 @@ struct Matrix<__bf16> {
 template <>
 struct Matrix<_Float16> {
   typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+  static constexpr float WEIGHT = 32768.f;  // the largest power of two that is a half
   static __device__ __forceinline__ f32x4 mul(V8 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -509,7 +515,7 @@ struct Tiles {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(s[h][r] - off);
+        const float p = Matrix<T>::WEIGHT * __builtin_amdgcn_exp2f(s[h][r] - off);
         l += p;
         hi[4 * h + r] = (T)p;
         lo[4 * h + r] = (T)(p - (float)hi[4 * h + r]);

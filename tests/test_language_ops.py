@@ -824,6 +824,44 @@ def test_attend_one_key_dominates(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0, 17.25, 19.0])
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,n", [
+    (2, 3, 1, 64, 61),       # one workgroup to an item
+    (1, 4, 2, 128, 5000),    # items shared by workgroups
+    (40, 16, 8, 128, 900),   # single waves as workers
+    (1030, 1, 1, 64, 500),   # one wave to an item
+])
+def test_attend_small_weights_count(device, dtype, gap, batch, heads, kv_heads, dim, n):
+    """A key of value 0 whose score lies ``gap`` above the others': the output
+    is what the small weights bring.  float16 weights are held times 2^15 in two
+    halves, so that each is off by half the smallest half, 2^-25, at most: 2^-40
+    of the largest weight."""
+    if device == "cpu" and batch > 2:
+        pytest.skip("the CPU form has no split")
+    g = gen(n)
+    page = 16
+    columns = -(-n // page)
+    lengths = [n] * batch
+    k_cache, v_cache, table = make_cache(g, batch, columns, kv_heads, page, dim, dtype, device)
+    k_cache.copy_(0.01 * torch.randn(k_cache.shape, generator=g))
+    v_cache.copy_(0.5 + torch.rand(v_cache.shape, generator=g))
+    for b in range(batch):
+        hot = (37 * b) % n
+        at = int(table[b, hot // page])
+        k_cache[at, :, hot % page] = 8 * gap / dim
+        v_cache[at, :, hot % page] = 0
+    q = torch.ones(batch, heads, dim, dtype=dtype, device=device)
+    out = ops.paged_attention_decode(
+        q, k_cache, v_cache, table, torch.tensor(lengths, device=device), scale=0.125)
+    some = sorted({0, batch // 2, batch - 1})
+    want, tol = attend_oracle(q[some], k_cache, v_cache, table[some], [n] * len(some), 0.125)
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -40 * n * 1.5
+    close(out[some], want, 1.01 * half_step(want, dtype) + tol)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_paged_refusals(device):
     k_cache = torch.zeros(4, 2, 8, 16, device=device)
     v_cache = torch.zeros_like(k_cache)
