@@ -462,6 +462,11 @@ __device__ __forceinline__ float kl3(float y) {
   return y * y * p;
 }
 
+// e^y - 1, which stays -1 for y down to -inf.
+__device__ __forceinline__ float kl3_slope(float y) {
+  return fabsf(y) > 0.5f ? exp2_hw(y * kLog2e) - 1.f : kl3(y) + y;
+}
+
 struct PolicyToken {
   bool above, below;
   double x;
@@ -519,10 +524,7 @@ __device__ __forceinline__ float policy_grad(const PolicyLossArgs& a, float lp, 
   const float dgain = a.variant == 0 ? (clipped_against(t, adv) ? 0.f : ratio * adv)
                                      : (t.above ? (float)a.high : t.below ? (float)a.low : ratio) * adv;
   float d = u.ge - u.go * dgain;
-  if (has_ref) {
-    const float y = ref - lp;
-    d -= u.gk * (kl3(y) + y);
-  }
+  if (has_ref) d -= u.gk * kl3_slope(ref - lp);
   return fmaf(d, w, e);
 }
 

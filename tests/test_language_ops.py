@@ -551,6 +551,32 @@ def test_policy_loss_second_derivative(device, variant, reduction):
     assert first.isfinite().all() and first[0, 0] == 0
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dense", [True, False])
+def test_policy_loss_kl_gradient_far_from_the_reference(device, dtype, dense):
+    """1 - e^y, y = ref - log_prob: -1 (times the coefficient) for a reference
+    that rules the token out, by infinity or the lowest value.  The exponent's
+    argument is off by u of its size, and two more roundings."""
+    low = torch.finfo(dtype).min
+    y = torch.tensor([-math.inf, low, -1e9, -3.5e7, -90.0, -30.0, -17.0, -5.0, -0.75, -0.5, 0.25, 0.5, 0.75, 5.0, 9.0])
+    ref = y.to(dtype)[None].repeat(3, 1)
+    old = torch.zeros_like(ref)
+    lp = torch.zeros_like(ref).to(device)
+    if not dense:
+        lp = lp.t().contiguous().t()
+    lp.requires_grad_()
+    out = ops.token_policy_loss(lp, old.to(device), torch.ones(3, 1, device=device), None, ref.to(device),
+                                kl_coeff=0.5, reduction="sum")
+    (grad,) = torch.autograd.grad(out.loss_kl, lp, retain_graph=True)
+    want = -0.5 * torch.expm1(ref.double())
+    tol = 0.5 * U * (ref.double().exp() * (4 + 3 * ref.double().abs().clamp(max=100)) + 4)
+    close(grad, want, tol + 1.01 * half_step(want, dtype))
+    # and as part of the whole: the objective's is -1
+    (grad,) = torch.autograd.grad(out.loss_total, lp)
+    close(grad, want - 1, tol + 4 * U + 1.01 * half_step(want - 1, dtype))
+
+
 # --------------------------------------------------------------------------- #
 # the paged cache
 # --------------------------------------------------------------------------- #
