@@ -480,7 +480,7 @@ Tensor policy_grad_plain(const Tensor& log_probs, const Tensor& old_log_probs,
                  ? ratio.masked_fill(against, 0)
                  : ratio.detach().masked_fill(above, 1 + c.high).masked_fill(below, 1 - c.low));
   Tensor d = (total + up(3)) * c.entropy - (total + up(1)) * dgain;
-  if (ref.defined()) d = d - (total + up(2)) * c.kl * kept(f64(ref) - lp).expm1();
+  if (ref.defined() && c.kl != 0) d = d - (total + up(2)) * c.kl * kept(f64(ref) - lp).expm1();
   d = kept(d * w * f64(factor));
   if (g[4].defined()) {
     const Tensor r = (f64(log_probs) - f64(old_log_probs)).exp();

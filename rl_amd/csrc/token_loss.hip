@@ -533,10 +533,12 @@ __device__ __forceinline__ void policy_finish(const PolicyLossArgs& a, const dou
   const double inv = a.mean ? 1.0 / (s[S_W] > 1.0 || isnan(s[S_W]) ? s[S_W] : 1.0) : 1.0;
   const double objective = -s[S_GAIN] * inv;
   const double kl = s[S_KL] * inv;
-  const double entropy = a.entropy_coeff * (s[S_LP] * inv);
-  a.out[0] = (float)(objective + a.kl_coeff * kl + entropy);
+  // a term without weight is left out: an infinite one times 0 would be NaN
+  const double loss_kl = a.kl_coeff == 0.0 ? 0.0 : a.kl_coeff * kl;
+  const double entropy = a.entropy_coeff == 0.0 ? 0.0 : a.entropy_coeff * (s[S_LP] * inv);
+  a.out[0] = (float)(objective + loss_kl + entropy);
   a.out[1] = (float)objective;
-  a.out[2] = (float)(a.kl_coeff * kl);
+  a.out[2] = (float)loss_kl;
   a.out[3] = (float)entropy;
   a.out[4] = (float)kl;
   a.out[5] = (float)(s[S_OFF] / n);

@@ -138,7 +138,8 @@ def token_policy_loss(
       ``loss_kl = kl_coeff * kl``;
     * ``loss_entropy``: ``entropy_coeff`` times the mean log-prob (the sampled
       entropy's negative);
-    * ``loss_total``: their sum;
+    * ``loss_total``: their sum; a term whose coefficient is 0 counts as 0,
+      infinite or not;
     * ``clip_fraction``: the share of all places, masked ones too, with
       ``|r - 1| > clip_low``; ``ess``: ``sum(r)^2 / sum(r^2) / numel`` over all
       places (as ``GRPOLoss`` reports them).
@@ -181,15 +182,20 @@ def token_policy_loss(
     gain = torch.minimum(ratio * adv, bounded * adv) if variant == "clip" else bounded.detach() * log_w * adv
     count = w.sum().clamp(min=1) if reduction == "mean" else 1.0
     objective = -(gain * w).sum() / count
-    kl = torch.zeros_like(objective)
+    # a term without weight is left out: 0 with a gradient of 0, whatever it holds
+    nothing = lp.masked_fill(torch.ones_like(gone), 0.0).sum()
+    kl, loss_kl, entropy = nothing.detach(), nothing, nothing
     if ref_log_probs is not None:
         y = torch.where(gone, 0.0, ref_log_probs.float() - lp)
         kl = ((torch.expm1(y) - y) * w).sum() / count
-    entropy = entropy_coeff * (lp * w).sum() / count
+        if kl_coeff != 0:
+            loss_kl = kl_coeff * kl
+    if entropy_coeff != 0:
+        entropy = entropy_coeff * (lp * w).sum() / count
     off = ((every.detach() - 1).abs() > clip_low).float().mean()
     ess = every.sum().square() / every.square().sum().clamp(min=1e-9) / every.numel()
     return TokenPolicyLoss(
-        objective + kl_coeff * kl + entropy, objective, kl_coeff * kl, entropy, kl.detach(), off, ess)
+        objective + loss_kl + entropy, objective, loss_kl, entropy, kl.detach(), off, ess)
 
 
 # --------------------------------------------------------------------------- #

@@ -577,6 +577,35 @@ def test_policy_loss_kl_gradient_far_from_the_reference(device, dtype, dense):
     close(grad, want - 1, tol + 4 * U + 1.01 * half_step(want - 1, dtype))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_policy_loss_terms_without_weight_are_left_out(device, create_graph):
+    """A term whose coefficient is 0 does not count, infinite or not; kl is still
+    reported, and every loss still has a gradient."""
+    old = torch.tensor([[-1.0, -2.0, -1.5]], device=device)
+    ref = torch.tensor([[-math.inf, math.inf, -1.0]], device=device)
+    adv = torch.ones(1, 1, device=device)
+
+    def grad(loss, lp):
+        return torch.autograd.grad(loss, lp, create_graph=create_graph, retain_graph=True)[0].detach()
+
+    lp = (old + 0.1).requires_grad_()
+    out = ops.token_policy_loss(lp, old, adv, None, ref, entropy_coeff=0.25)
+    assert not out.kl.isfinite() and out.loss_kl == 0  # inf - inf
+    assert abs(float(out.loss_total.detach() - out.loss_objective.detach() - out.loss_entropy.detach())) <= 4 * U
+    want = (0.25 - (lp.detach() - old).exp()) / 3
+    assert ((grad(out.loss_total, lp) - want).abs() <= 16 * U).all()
+    assert (grad(out.loss_kl, lp) == 0).all()
+    # no reference at all, and a log-prob of -inf without an entropy term
+    lp = torch.tensor([[-1.0, -math.inf, -1.5]], device=device, requires_grad=True)
+    out = ops.token_policy_loss(lp, old, adv)
+    assert out.loss_entropy == 0 and out.loss_kl == 0 and out.kl == 0
+    assert out.loss_total == out.loss_objective and out.loss_total.isfinite()
+    want = torch.tensor([[-1.0, 0.0, -1.0]], device=device) / 3
+    assert ((grad(out.loss_total, lp) - want).abs() <= 16 * U).all()
+    assert (grad(out.loss_kl, lp) == 0).all() and (grad(out.loss_entropy, lp) == 0).all()
+
+
 # --------------------------------------------------------------------------- #
 # the paged cache
 # --------------------------------------------------------------------------- #
