@@ -175,6 +175,8 @@ void per_sequence(const char* op, const Tensor& t, const char* name, int64_t bat
 void no_grad(const char* op, const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), op, ": ", name,
                     " requires a gradient, and this operator has none: call it under torch.no_grad()");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), op, ": ", name,
+                    " carries a forward derivative, and this operator has none");
 }
 
 using Rope = std::optional<std::tuple<Tensor, Tensor>>;

@@ -32,11 +32,16 @@ __all__ = [
 ]
 
 _VARIANTS = {"clip": 0, "cispo": 1}
+_fw = torch.autograd.forward_ad
 
 
-def _native(tensor: torch.Tensor):
+def _native(tensor: torch.Tensor, *others: Optional[torch.Tensor]):
     """The extension for a GPU tensor; None on the CPU (and on a GPU without
-    it where the eager fallback is allowed)."""
+    it where the eager fallback is allowed), and where one of the tensors carries a
+    forward derivative, which the kernels do not compute."""
+    if _fw._current_level >= 0 and any(
+            t is not None and _fw.unpack_dual(t).tangent is not None for t in (tensor, *others)):
+        return None
     return _C if tensor.is_cuda and _require_ext() else None
 
 
@@ -44,7 +49,7 @@ def _ordinary(*tensors: torch.Tensor) -> bool:
     """Whether all are tensors whose memory a kernel can take: not subclasses,
     not under functorch's transforms, forward derivatives or a tracing compiler.
     What offers an operator in place of elementary torch asks this first."""
-    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level >= 0:
+    if torch.compiler.is_compiling() or _fw._current_level >= 0:
         return False
     return all(
         type(t) in (torch.Tensor, torch.nn.Parameter)
@@ -77,7 +82,7 @@ def token_log_probs(
     Returns:
         ``[...]`` float32.  Differentiable in ``logits``; the gradient has
         the logits' dtype, and is itself differentiable in elementary operations
-        (``create_graph``).  A place with an upstream gradient of 0 gets a
+        (``create_graph``); forward derivatives (dual tensors) take these as well.  A place with an upstream gradient of 0 gets a
         gradient of exactly 0 whatever its logits hold.  A row of nothing but
         ``-inf`` gives NaN.
     """
@@ -101,7 +106,8 @@ def token_log_probs(
 # --------------------------------------------------------------------------- #
 class TokenPolicyLoss(NamedTuple):
     """What :func:`token_policy_loss` returns: float32 scalars.  The first
-    four and ``ess`` carry a gradient to ``log_probs``."""
+    four and ``ess`` carry a gradient to ``log_probs``, and the forward derivatives
+    of dual tensors, in elementary operations."""
 
     loss_total: torch.Tensor
     loss_objective: torch.Tensor
@@ -159,7 +165,7 @@ def token_policy_loss(
         raise ValueError(f"token_policy_loss: variant must be one of {sorted(_VARIANTS)}, got {variant!r}")
     if reduction not in ("mean", "sum"):
         raise ValueError(f"token_policy_loss: reduction must be 'mean' or 'sum', got {reduction!r}")
-    c = _native(log_probs)
+    c = _native(log_probs, old_log_probs, advantage, mask, ref_log_probs)
     if c is not None:
         return TokenPolicyLoss(*c.token_policy_loss(
             log_probs, old_log_probs, advantage, mask, ref_log_probs, _VARIANTS[variant],

@@ -984,3 +984,43 @@ def test_paged_refusals(device):
     if device == "cuda":
         with pytest.raises(ValueError, match="is on"):
             attend(n=start.cpu())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_derivatives(device):
+    """A direct call's tangent is the gradient's product with it; what has no
+    derivative refuses one."""
+    fw = torch.autograd.forward_ad
+    g = gen(21)
+    logits, t = torch.randn(2, 3, 5, 17, generator=g).to(device)
+    tokens = torch.randint(0, 17, (3, 5), generator=g).to(device)
+    lp, tlp, old, ref = torch.randn(4, 3, 5, generator=g).to(device)
+    adv = torch.randn(3, 1, generator=g).to(device)
+
+    def losses(x):
+        out = ops.token_policy_loss(x, old, adv, None, ref, kl_coeff=0.1, entropy_coeff=0.2)
+        return [*out[:4], out.ess]
+
+    leaf = logits.clone().requires_grad_()
+    value = ops.token_log_probs(leaf, tokens)
+    want = torch.stack([(torch.autograd.grad(v, leaf, retain_graph=True)[0] * t).sum()
+                        for v in value.flatten()]).view(3, 5)
+    with fw.dual_level():
+        got = fw.unpack_dual(ops.token_log_probs(fw.make_dual(logits, t), tokens))
+        assert got.tangent is not None and torch.allclose(got.tangent, want, atol=1e-5)
+        assert torch.allclose(got.primal, value, atol=1e-5)
+        # a level by itself changes nothing
+        assert torch.equal(ops.token_log_probs(logits, tokens), value)
+        x = lp.clone().requires_grad_()
+        for got, one in zip(losses(fw.make_dual(lp, tlp)), losses(x)):
+            (want,) = torch.autograd.grad(one, x, retain_graph=True)
+            assert torch.allclose(fw.unpack_dual(got).tangent, (want * tlp).sum(), atol=1e-4)
+        k_cache, v_cache = torch.zeros(2, 4, 1, 8, 16, device=device)
+        table = torch.zeros(3, 1, dtype=torch.int32, device=device)
+        start = torch.zeros(3, dtype=torch.int32, device=device)
+        k = torch.zeros(3, 1, 1, 16, device=device)
+        dual = fw.make_dual(k, k)
+        with pytest.raises(ValueError, match="derivative"), torch.no_grad():
+            ops.paged_kv_append(dual, k, k_cache, v_cache, table, start)
+        with pytest.raises(ValueError, match="derivative"):
+            ops.paged_attention_decode(dual[:, 0], k_cache, v_cache, table, start)
