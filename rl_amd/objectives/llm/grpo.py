@@ -88,6 +88,9 @@ class GRPOLoss(LossModule):
     def _fused_clip(self):
         return "clip", self.clip_epsilon, self.clip_epsilon
 
+    _MASK_DTYPES = (torch.bool, torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64,
+                    torch.float16, torch.bfloat16, torch.float32)
+
     @staticmethod
     def _broadcasts(x, to) -> bool:
         return x.dim() <= to.dim() and all(
@@ -112,7 +115,8 @@ class GRPOLoss(LossModule):
             or not self._broadcasts(adv, new_lp)
             or any(t.dtype not in (torch.float32, torch.bfloat16, torch.float16)
                    for t in (new_lp, old_lp, adv) + (() if ref_lp is None else (ref_lp,)))
-            or (mask is not None and mask.is_complex())
+            # masks of more bits than the kernel reads: float64 sums stay float64
+            or (mask is not None and mask.dtype not in self._MASK_DTYPES)
         ):
             return None
         variant, low, high = self._fused_clip()

@@ -155,7 +155,7 @@ def token_policy_loss(
             or float16, any strides.  Only ``log_probs`` gets a gradient; the
             others must not require one.
         advantage: broadcasts to ``log_probs``.
-        mask: bool, integer or float weights of ``log_probs``' shape.  A place
+        mask: bool, integer or float weights of ``log_probs``' shape, taken in float32.  A place
             of weight 0 may hold anything (the losses' gradient there is 0),
             though what it holds still enters ``clip_fraction`` and ``ess``.
         reduction: ``"mean"`` as above, or ``"sum"``: the weighted sums, not

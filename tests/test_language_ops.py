@@ -413,6 +413,28 @@ def test_policy_loss_masked_places_hold_anything(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("mask_dtype", [torch.bool, torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64,
+                                        torch.float16, torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("shape", [(3, 8), (7, 5), (130, 257)])
+def test_policy_loss_mask_types(device, mask_dtype, shape):
+    """Weights 0, 1 and, where the type has them, 2 and -1: sums of float32
+    terms of size 10, each off by some 16 u."""
+    g = gen(31)
+    old = -torch.rand(shape, generator=g) * 2
+    lp = old + 0.3 * torch.randn(shape, generator=g)
+    adv = torch.randn(shape[0], 1, generator=g)
+    mask = torch.randint(0 if mask_dtype in (torch.bool, torch.uint8) else -1, 3, shape, generator=g).to(mask_dtype)
+    x = lp.to(device).requires_grad_()
+    out = ops.token_policy_loss(x, old.to(device), adv.to(device), mask.to(device), reduction="sum",
+                                entropy_coeff=0.1)
+    (grad,) = torch.autograd.grad(out.loss_total, x)
+    want, _, _ = policy_oracle(lp, old, adv, mask, None, 0.2, 0.2, "clip", 0.0, 0.1, "sum")
+    n = lp.numel()
+    assert abs(float(out.loss_total.detach()) - float(want["loss_total"])) <= 16 * U * 10 * n
+    close(grad, want["grad"], 64 * U * (want["grad"].abs() + 1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_policy_loss_outputs_change_in_place(device):
     lp = torch.zeros(2, 3, device=device, requires_grad=True)
     out = ops.token_policy_loss(lp, torch.zeros(2, 3, device=device), torch.ones(2, 1, device=device))

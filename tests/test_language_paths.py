@@ -432,6 +432,47 @@ def test_grpo_results_have_the_plain_forms_types(new, old, adv, ref, mask, autoc
         assert {k: got.get(k).dtype for k in got.keys()} == {k: want.get(k).dtype for k in want.keys()}
 
 
+def plain_of(cls):
+    """The loss class with its gain overridden by itself: the plain form."""
+    return type("Plain" + cls.__name__, (cls,), {"_ratio_clip_gain": lambda self, x, a: cls._ratio_clip_gain(self, x, a)})
+
+
+def grpo_data(seed=9, shape=(5, 17)):
+    g = torch.Generator().manual_seed(seed)
+    old = -torch.rand(shape, generator=g) * 3
+    return dict(new=(old + 0.4 * torch.randn(shape, generator=g)).cuda(), old=old.cuda(),
+                adv=torch.randn(shape[0], 1, generator=g).cuda(),
+                ref=(old + 0.2 * torch.randn(shape, generator=g)).cuda(),
+                mask=torch.rand(shape, generator=g).cuda())
+
+
+def grpo_td(d, mask):
+    return TensorDict({"log_probs": d["old"], "advantage": d["adv"], "ref_log_probs": d["ref"],
+                       "attention_mask_response": mask}, batch_size=[d["old"].shape[0]])
+
+
+def both_forms(cls, d, mask, **kw):
+    res = []
+    for c in (cls, plain_of(cls)):
+        lp = d["new"].clone().requires_grad_()
+        vals = c(Given(lp), kl_to_ref_coeff=0.1, entropy_coeff=0.02, **kw)(grpo_td(d, mask))
+        (grad,) = torch.autograd.grad(sum(vals.get(k) for k in vals.keys() if k.startswith("loss")), lp)
+        res.append(({k: vals.get(k).detach() for k in vals.keys()}, grad))
+    return res
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loss_cls", [GRPOLoss, DAPO, CISPOLoss])
+def test_grpo_float64_masks_keep_float64(loss_cls):
+    """The plain form multiplies and sums in the mask's 64 bits."""
+    d = grpo_data()
+    (got, grad), (want, dwant) = both_forms(loss_cls, d, d["mask"].double() / 3)
+    for k in want:
+        assert got[k].dtype == want[k].dtype
+        assert abs(float(got[k] - want[k])) <= 2.0 ** -44 * max(1.0, abs(float(want[k]))), k
+    assert torch.allclose(grad, dwant, rtol=1e-5, atol=1e-7)
+
+
 @pytest.mark.gpu
 def test_wrapper_log_probs_under_autocast():
     from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
