@@ -6,6 +6,7 @@ DAPO:953, CISPOLoss:1004, MCAdvantage:1028), sft.py:104.
 from __future__ import annotations
 
 import dataclasses
+import math
 from typing import Optional
 
 import torch
@@ -121,7 +122,8 @@ class GRPOLoss(LossModule):
             return None
         variant, low, high = self._fused_clip()
         coeffs = (low, high, self.entropy_coeff or 0.0, self.kl_to_ref_coeff or 0.0)
-        if not all(isinstance(x, (int, float)) for x in coeffs) or low < 0 or high < 0:
+        # (an infinite bound, for no clipping on that side, is the plain form's)
+        if not all(isinstance(x, (int, float)) and math.isfinite(x) for x in coeffs) or low < 0 or high < 0:
             return None
         loss = ops.token_policy_loss(
             new_lp, old_lp, adv, mask, ref_lp, clip_low=low, clip_high=high, variant=variant,

@@ -474,6 +474,20 @@ def test_grpo_float64_masks_keep_float64(loss_cls):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("loss_cls,kw", [
+    (GRPOLoss, dict(clip_epsilon=math.inf)), (CISPOLoss, dict(clip_epsilon=math.inf)),
+    (DAPO, dict(clip_epsilon_high=math.inf)), (DAPO, dict(clip_epsilon_low=math.inf, clip_epsilon_high=math.inf)),
+])
+def test_grpo_without_clip_bounds(loss_cls, kw):
+    """An infinite bound means no clipping on that side."""
+    d = grpo_data()
+    (got, grad), (want, dwant) = both_forms(loss_cls, d, d["mask"] < 0.7, **kw)
+    for k in want:
+        assert torch.allclose(got[k], want[k], atol=1e-5), k
+    assert torch.allclose(grad, dwant, atol=1e-6)
+
+
+@pytest.mark.gpu
 def test_wrapper_log_probs_under_autocast():
     from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
 
