@@ -47,9 +47,15 @@ def _native(tensor: torch.Tensor, *others: Optional[torch.Tensor]):
 
 def _ordinary(*tensors: torch.Tensor) -> bool:
     """Whether all are tensors whose memory a kernel can take: not subclasses,
-    not under functorch's transforms, forward derivatives or a tracing compiler.
-    What offers an operator in place of elementary torch asks this first."""
-    if torch.compiler.is_compiling() or _fw._current_level >= 0:
+    not under functorch's transforms, forward derivatives, a tracing compiler, a
+    trace or a mode that sees every operation.  What offers an operator in place of
+    elementary torch asks this first."""
+    if (
+        torch.compiler.is_compiling()
+        or _fw._current_level >= 0
+        or torch.jit.is_tracing()
+        or torch._C._len_torch_dispatch_stack()
+    ):
         return False
     return all(
         type(t) in (torch.Tensor, torch.nn.Parameter)

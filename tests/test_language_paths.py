@@ -540,6 +540,41 @@ def test_transforms_and_subclasses_keep_the_plain_form():
     assert type(_log_probs_of(logits.as_subclass(Wrapped), tokens)) is Wrapped
 
 
+@pytest.mark.gpu
+def test_tracers_and_dispatch_modes_keep_the_plain_form():
+    """A trace records the loss's operations, not one call's numbers; modes that
+    see every operation see the loss's."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
+
+    d = grpo_data()
+    td = grpo_td(d, d["mask"] < 0.7)
+
+    def loss(x):
+        return GRPOLoss(Given(x))(td).get("loss_objective")
+
+    traced = torch.jit.trace(loss, (d["new"],))
+    other = d["new"] + 0.1
+    assert torch.allclose(traced(other), loss(other), atol=1e-6)
+    logits = torch.randn(2, 5, 11, generator=torch.Generator().manual_seed(3)).cuda()
+    tokens = torch.randint(0, 11, (2, 5), generator=torch.Generator().manual_seed(4)).cuda()
+    traced = torch.jit.trace(_log_probs_of, (logits, tokens))
+    assert torch.allclose(traced(logits * 2, tokens), _log_probs_of(logits * 2, tokens), atol=1e-5)
+
+    class Seen(TorchDispatchMode):
+        names = ()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names += (str(func),)
+            return func(*args, **(kwargs or {}))
+
+    for call in (lambda: loss(d["new"]), lambda: _log_probs_of(logits, tokens)):
+        with Seen() as mode:
+            call()
+        assert any("exp" in n or "log_softmax" in n for n in mode.names)
+
+
 # --------------------------------------------------------------------------- #
 # streams, graphs, far offsets
 # --------------------------------------------------------------------------- #
