@@ -25,6 +25,7 @@ def _log_probs_of(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     autocast, as ``log_softmax`` itself)."""
     if (
         logits.is_cuda
+        and tokens.shape == logits.shape[:-1]  # gather takes fewer rows as well
         and logits.dtype in (torch.float32, torch.bfloat16, torch.float16)
         and _ordinary(logits, tokens)
     ):

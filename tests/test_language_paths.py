@@ -500,6 +500,20 @@ def test_wrapper_log_probs_under_autocast():
     assert (got - want).abs().max() <= 64 * U * 10
 
 
+@pytest.mark.gpu
+def test_wrapper_log_probs_of_fewer_tokens_than_rows():
+    """Beam search scores more rows than it returns sequences: the rows that
+    have a token are taken, as indexing does."""
+    from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
+
+    g = torch.Generator().manual_seed(5)
+    scores = torch.randn(6, 503, generator=g).cuda()
+    tokens = torch.randint(0, 503, (2,), generator=g).cuda()
+    got = _log_probs_of(scores, tokens)
+    want = scores[:2].double().log_softmax(-1).gather(-1, tokens[:, None]).squeeze(-1)
+    assert got.shape == (2,) and (got.double() - want).abs().max() <= 64 * U * 10
+
+
 class Wrapped(torch.Tensor):
     """A subclass that sees every operation on it, as sharded tensors do."""
 
