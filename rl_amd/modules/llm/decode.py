@@ -225,7 +225,8 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
     produced ``eos_token_id`` stops writing to its cache.
 
     Args:
-        model: a transformers GPT-2 with LM head.
+        model: a transformers GPT-2 with tied LM head, tanh GELU and attention
+            scores over ``sqrt(dim)`` (the architecture's defaults).
         batch: sequences per rollout.
         max_len: longest prompt plus response; at most the model's positions.
         temperature: of the sampling and of the recorded log-probs.
@@ -238,6 +239,18 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         if max_len > model.config.n_positions:
             raise ValueError(
                 f"PagedGPT2Decoder: max_len {max_len} exceeds the model's {model.config.n_positions} positions")
+        c = model.config
+        if (
+            c.activation_function not in self._TANH_GELU
+            or not c.scale_attn_weights
+            or c.scale_attn_by_inverse_layer_idx
+        ):
+            raise ValueError(
+                "PagedGPT2Decoder: the decode step is that of a tanh GELU and scores over sqrt(dim), not of "
+                f"activation_function={c.activation_function!r}, scale_attn_weights={c.scale_attn_weights}, "
+                f"scale_attn_by_inverse_layer_idx={c.scale_attn_by_inverse_layer_idx}")
+        if model.lm_head.weight.data_ptr() != model.transformer.wte.weight.data_ptr():
+            raise ValueError("PagedGPT2Decoder: the LM head must be tied to the token embedding")
         if eos_token_id is not None and not 0 <= eos_token_id < model.config.vocab_size:
             raise ValueError(
                 f"PagedGPT2Decoder: eos_token_id {eos_token_id} is not in the vocabulary of {model.config.vocab_size}")
@@ -261,6 +274,7 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         self._graph = None
 
     _CHUNK = 512
+    _TANH_GELU = ("gelu_new", "gelu_pytorch_tanh", "gelu_fast", "gelu_accurate")
 
     def _draw(self, logits: torch.Tensor) -> torch.Tensor:
         """A token of ``softmax(logits / temperature)`` per row: the argmax of

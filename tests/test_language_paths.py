@@ -256,6 +256,20 @@ def test_paged_rollout_refusals():
             dec.rollout(prompts, 4, torch.tensor(bad))
 
 
+@pytest.mark.parametrize("kw", [
+    dict(activation_function="relu"), dict(activation_function="gelu"),
+    dict(scale_attn_by_inverse_layer_idx=True), dict(scale_attn_weights=False),
+    dict(tie_word_embeddings=False),
+])
+def test_paged_rollout_refuses_models_it_does_not_compute(kw):
+    """The decode step is GPT-2's with tanh GELU, 1 / sqrt(dim) and a tied head;
+    a model of another kind would be decoded wrongly."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    with pytest.raises(ValueError, match=next(iter(kw)) if "tie" not in next(iter(kw)) else "tied"):
+        PagedGPT2Decoder(make_lm(**kw), 2, 20, "cpu", dtype=torch.float32)
+
+
 @pytest.mark.gpu
 def test_paged_rollout_matches_hf_bf16():
     """bf16, mixed prompt lengths: the next-token logits of the HF model."""
