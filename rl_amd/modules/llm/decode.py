@@ -221,6 +221,7 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
     (:func:`rl_amd.ops.paged_kv_append`) and one attention over each
     sequence's own length (:func:`rl_amd.ops.paged_attention_decode`), where
     :class:`GraphedGPT2Decoder` attends over ``max_len`` for every sequence.
+    There is no dropout, whatever mode the model is in.
     After :meth:`capture` each token is one graph replay; a sequence that has
     produced ``eos_token_id`` stops writing to its cache.
 
@@ -353,12 +354,20 @@ class PagedGPT2Decoder(GraphedGPT2Decoder):
         self.cache.reset()
         self.cache.reserve([self.T] * B)
         count = lengths.to(device=self.device, dtype=torch.int32)
-        with torch.no_grad(), torch.autocast(
-            "cuda", dtype=self.dtype, cache_enabled=False, enabled=prompts.is_cuda,
-        ):
-            out = self._tr(input_ids=prompts, use_cache=True)
-            last = out.last_hidden_state[torch.arange(B, device=prompts.device), count.long() - 1]
-            logits = self.model.lm_head(last).float()
+        # the decode step has no dropout, so the prompt gets none either
+        training = [m for m in self._tr.modules() if m.training]
+        try:
+            for m in training:
+                m.training = False
+            with torch.no_grad(), torch.autocast(
+                "cuda", dtype=self.dtype, cache_enabled=False, enabled=prompts.is_cuda,
+            ):
+                out = self._tr(input_ids=prompts, use_cache=True)
+                last = out.last_hidden_state[torch.arange(B, device=prompts.device), count.long() - 1]
+                logits = self.model.lm_head(last).float()
+        finally:
+            for m in training:
+                m.training = True
         past = out.past_key_values
         self.cache.extend(count)
         with torch.no_grad():

@@ -270,6 +270,25 @@ def test_paged_rollout_refuses_models_it_does_not_compute(kw):
         PagedGPT2Decoder(make_lm(**kw), 2, 20, "cpu", dtype=torch.float32)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_paged_rollout_has_no_dropout(device):
+    """A policy in training mode is decoded without dropout, the prompt too: the
+    log-probs are the evaluated model's, and the modules' modes stay."""
+    from rl_amd.modules.llm import PagedGPT2Decoder
+
+    model = make_lm(resid_pdrop=0.5, embd_pdrop=0.5, attn_pdrop=0.5).to(device)
+    dec = PagedGPT2Decoder(model, 4, 40, device, dtype=torch.float32)
+    model.train()
+    model.transformer.h[1].eval()
+    modes = [m.training for m in model.modules()]
+    torch.manual_seed(0)
+    prompts, lengths = ragged_prompts(device)
+    out = dec.rollout(prompts, 6, lengths)
+    assert [m.training for m in model.modules()] == modes
+    want = hf_log_probs(model.eval(), prompts, lengths, out, 1.0)
+    assert (out.get("log_probs").cpu().double() - want).abs().max() < 2e-4
+
+
 @pytest.mark.gpu
 def test_paged_rollout_matches_hf_bf16():
     """bf16, mixed prompt lengths: the next-token logits of the HF model."""
