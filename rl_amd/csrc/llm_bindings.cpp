@@ -659,7 +659,12 @@ OptTensor paged_kv_append(const Tensor& k_in, const Tensor& v_in, const Tensor& 
            a.rotary / 2 % wide == 0;
   };
   while (a.vec > 1 && !fits(a.vec)) a.vec = a.vec > 4 ? 4 : 1;
-  if (a.batch * a.width) launched(launch_paged_append(&a, stream_of()), "paged_kv_append");
+  if (a.batch * a.width) {
+    launched(launch_paged_append(&a, stream_of()), "paged_kv_append");
+    // what autograd has saved of the caches is no longer what it was
+    for (const Tensor* t : {&k_cache, &v_cache})
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
   return q_in ? OptTensor(q_out) : std::nullopt;
 }
 

@@ -708,6 +708,30 @@ def test_append(device, dtype, batch, width, heads, kv_heads, dim, page, rotary,
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_append_is_an_in_place_change(device):
+    """A cache that an earlier operation keeps for its backward pass: the
+    backward pass refuses, as after any other change in place.  Inference
+    tensors, which have no version, are written as before."""
+    def case():
+        k_cache = torch.zeros(4, 1, 8, 16, device=device)
+        return k_cache, torch.zeros_like(k_cache), torch.ones(2, 1, 1, 16, device=device)
+
+    table = torch.tensor([[1], [3]], dtype=torch.int32, device=device)
+    start = torch.zeros(2, dtype=torch.int32, device=device)
+    for which in (0, 1):
+        caches = case()
+        w = torch.ones((), device=device, requires_grad=True)
+        loss = (w * caches[which]).sum()
+        ops.paged_kv_append(caches[2], caches[2], caches[0], caches[1], table, start)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        k_cache, v_cache, k = case()
+        ops.paged_kv_append(k, k, k_cache, v_cache, table, start)
+        assert (k_cache[1, 0, 0] == 1).all() and (k_cache[0] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_append_bad_places_write_nothing(device):
     g = gen(1)
     k_cache, v_cache, _ = make_cache(g, 6, 1, 2, 8, 16, torch.float32, device)
