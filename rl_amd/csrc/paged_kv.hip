@@ -1152,7 +1152,8 @@ extern "C" void plan_paged_attend(PagedAttendArgs* a, int cus) {
   const int size = a->dtype == RL_F32 ? 4 : 2;
   const int keys = size == 4 ? 16 : 32;
   const long room = (long)a->cache.table_cols << a->cache.page_shift;
-  const long most = (room + keys - 1) / keys;  // tiles of an item
+  // tiles of an item, one at least: no pages at all are an empty item's one tile
+  const long most = room > 0 ? (room + keys - 1) / keys : 1;
   const int group = a->heads / a->kv_heads;
   a->head_blocks = (group + 15) / 16;
   const long items = a->batch * a->kv_heads * a->head_blocks;

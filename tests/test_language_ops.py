@@ -869,6 +869,25 @@ def test_attend_batches(dtype, batch, longest, heads, kv_heads, dim, page):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batch", [65535, 65536, 70001])
+def test_attend_many_sequences(device, batch):
+    """More sequences than a grid's second axis takes, without a page and with
+    one of a few keys: a key of its own for each third sequence."""
+    k_cache = torch.zeros(3, 1, 8, 8, device=device)
+    k_cache[1:] = 1.0
+    v_cache = torch.arange(24.0, device=device).view(3, 1, 8, 1).expand(-1, -1, -1, 8).contiguous()
+    q = torch.zeros(batch, 1, 8, device=device)
+    lengths = torch.arange(batch, device=device) % 3
+    none = torch.zeros(batch, 0, dtype=torch.int32, device=device)
+    assert (ops.paged_attention_decode(q, k_cache, v_cache, none, lengths) == 0).all()
+    table = (torch.arange(batch, device=device) % 2).int()[:, None]
+    out = ops.paged_attention_decode(q, k_cache, v_cache, table, lengths)
+    # no key: 0; one: the page's first value; two: the mean of its first two
+    want = torch.where(lengths == 0, 0.0, 8.0 * table[:, 0] + 0.5 * (lengths - 1))
+    assert torch.equal(out[:, 0], want[:, None].expand(-1, 8))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_bad_pages_and_layouts(device, dtype):
     """Missing pages are left out, a length past the table is cut, layer views
