@@ -701,10 +701,11 @@ Tensor paged_attention_decode(const Tensor& q_in, const Tensor& k_cache, const T
   if (a.workers) {
     const int64_t rows = 2 * (int64_t)a.workers * std::min(16, a.heads / a.kv_heads);
     const int64_t notes = a.workers * paged_attend_note_bytes() / 4;
-    part = torch::empty({notes + rows * (a.dim + 2)}, q.options().dtype(torch::kFloat32));
-    a.notes = part.data_ptr<float>();
-    a.part = part.data_ptr<float>() + notes;
+    part = torch::empty({rows * (a.dim + 2) + notes}, q.options().dtype(torch::kFloat32));
+    // widest accesses first: rows is even and dim a multiple of 8, so all are aligned
+    a.part = part.data_ptr<float>();
     a.part_ms = a.part + rows * a.dim;
+    a.notes = a.part_ms + rows * 2;
   }
   launched(launch_paged_attend(&a, stream_of()), "paged_attention_decode");
   return out;

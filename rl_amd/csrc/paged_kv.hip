@@ -1186,6 +1186,9 @@ extern "C" int launch_paged_append(const PagedAppendArgs* a, void* stream) {
 
 extern "C" int launch_paged_attend(const PagedAttendArgs* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
+  // the parts are written and read 16 bytes at a time, the notes hold 8-byte numbers
+  if (a->workers && ((size_t)a->part % 16 != 0 || (size_t)a->notes % 8 != 0))
+    return (int)hipErrorInvalidValue;
   switch (a->dtype) {
     case RL_F32:
       return attend_any<float>(*a, st);

@@ -887,6 +887,24 @@ def test_attend_many_sequences(device, batch):
     assert torch.equal(out[:, 0], want[:, None].expand(-1, 8))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tiles", [17, 21, 33])
+def test_attend_odd_workers(dtype, tiles):
+    """One item shared by an odd number of workgroups (a fourth of its tiles,
+    rounded up): the parts' wide accesses are aligned."""
+    g = gen(tiles)
+    keys = 16 if dtype == torch.float32 else 32
+    n = keys * tiles - 3
+    k_cache, v_cache, table = make_cache(g, 1, -(-n // 16), 1, 16, 128, dtype, "cuda")
+    fill_cache(g, k_cache, table, [n])
+    fill_cache(g, v_cache, table, [n])
+    q = torch.randn(1, 5, 128, generator=g).to(dtype).cuda()
+    out = ops.paged_attention_decode(q, k_cache, v_cache, table, torch.tensor([n], device="cuda"))
+    want, tol = attend_oracle(q, k_cache, v_cache, table, [n], 128 ** -0.5)
+    close(out, want, 1.01 * half_step(want, dtype) + tol)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_bad_pages_and_layouts(device, dtype):
