@@ -4,6 +4,7 @@ In-tree build: ``python setup.py build_ext --inplace`` produces
 ``rl_amd/_C*.so`` next to the package so it ships with the source tree.
 Target arch is gfx950 only (MI355X) — set via PYTORCH_ROCM_ARCH.
 """
+import glob
 import os
 import sys
 
@@ -18,6 +19,14 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "rl_amd", "csrc")
 
 with_hip = torch.version.hip is not None
+
+# Objects that hipcc made know no headers: what is older than one is compiled again
+# (the two sides of a launch must agree on its structs).
+headers = glob.glob(os.path.join(CSRC, "*.h"))
+newest = max((os.path.getmtime(h) for h in headers), default=0.0)
+for obj in glob.glob(os.path.join(ROOT, "build", "temp*", "**", "*.o"), recursive=True):
+    if os.path.getmtime(obj) < newest:
+        os.remove(obj)
 
 sources = [
     os.path.join(CSRC, "bindings.cpp"),
@@ -63,6 +72,7 @@ setup(
         ext_cls(
             name="rl_amd._C",
             sources=sources,
+            depends=headers,
             define_macros=define_macros,
             **extra,
         )
