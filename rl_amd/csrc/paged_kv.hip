@@ -230,7 +230,9 @@ int append_vec(const PagedAppendArgs& a, hipStream_t st) {
 // Measured (one MI355X, where a large copy runs at 4.9 TB/s): 1 x 131072 keys, 32 +
 // 8 heads of 128 bf16, 98 us a call, 93 in the kernel (5.8 TB/s) and 5 in the join;
 // 48 sequences of 1 to 8192 keys 152 us (5.3 TB/s); 256 of 65 to 96 keys, 12 heads of
-// 64, 13.5 us (4.7 TB/s).  Bound by HBM; small calls by three dependent loads (length,
+// 64, 13.3 us (4.7 TB/s).  float32: 48 of 1 to 4096 keys, 32 + 8 heads of 128, 161 us
+// (5.0 TB/s); 65536 keys 121 us (4.5 TB/s); 256 of 65 to 96, 12 heads of 64, 27 us (4.7
+// TB/s).  Bound by HBM; small calls by three dependent loads (length,
 // page id, key) and the launch.
 // ---------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -1137,10 +1139,12 @@ extern "C" long paged_attend_note_bytes(void) { return (long)sizeof(SharedItem);
 //   13.6 / 13.5]; of dim 128, 300 / 500 / 800: 10.6 / 13.3 / 18.2 [14.5 / 13.0 / 14.9];
 //   200 items of dim 64, 800: 14 [19].  With single waves, up to 16 tiles: 2048 items
 //   of 16 tiles, dim 128, 100 [106]; 4096 of 4 57 [65].
-// - From 256 items on a worker is one wave, below a workgroup of four: ragged
-//   lengths of 1 to 1024, 768 items of dim 64, 28 [51]; 512 of dim 128 39 [64]; 1
-//   to 8192, 384 of dim 128, 160 [171]; but 16 items of 1 to 30000 38 [45], 8 of
-//   131072 101 [114].  Equal lengths gain less or lose: 384 items of 4096 153 [144].
+// - From 256 items on a worker is one wave, below a workgroup of four.  Ragged lengths of
+//   1 to 8192, dim 128, 256 items 119 [130], 384 items 172 [184]; of 1 to 1024, 512 items
+//   36 [60]; of 100 to 700, dim 64, 2048 items 54 [70].  Equal lengths are even: 384 items
+//   of 4096, dim 128, 151 [154], 256 items 113 [112].  But 16 items of 1 to 30000 34 [83],
+//   8 of 131072 105 [164].  In between single waves would do from some 128 items on: 128
+//   and 192 items of 1 to 8192 81 and 108 [71 and 97].
 // - Workers are as many as fill the card once, no more: each has a start of its
 //   own, and shares items that must be joined.  Single waves two to a SIMD: 512
 //   items of 1 to 1024, dim 128, 41 [49 with one, 44 with three].  Workgroups one

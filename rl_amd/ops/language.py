@@ -339,7 +339,8 @@ def paged_attention_decode(
         scale: default ``dim ** -0.5``.
 
     Keys on pages outside ``[0, pages)`` are left out; slots past a sequence's
-    length may hold anything.
+    length may hold anything.  What counts has to be finite: an infinite value gives
+    infinity or NaN.
 
     Returns:
         ``[batch, heads, dim]`` in ``q``'s dtype.
