@@ -334,7 +334,9 @@ def main():
                         "kl_to_ref": "k3",
                         "decode": ("graph" if decode_graph is not None
                                    else "static" if use_static
-                                   else "paged" if fused else "generate"),
+                                   else "graphdec" if graphdec is not None
+                                   else args.decode_mode if args.decode_mode in ("manual", "paged")
+                                   else "generate"),
                     },
                 }
             )
