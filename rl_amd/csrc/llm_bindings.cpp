@@ -230,6 +230,7 @@ void paged_kv_append_check(const Tensor& k, const Tensor& v, const Tensor& k_cac
                        t->scalar_type());
       TORCH_CHECK_VALUE(t->is_contiguous(), op, ": rope must be contiguous");
       same_device(k_cache, *t, op, "rope");
+      no_grad(op, *t, "rope");
     }
   } else {
     TORCH_CHECK_VALUE(!q, op, ": q is taken to be rotated, and there is no rope");

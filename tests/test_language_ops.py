@@ -1107,3 +1107,20 @@ def test_forward_derivatives(device):
             ops.paged_kv_append(dual, k, k_cache, v_cache, table, start)
         with pytest.raises(ValueError, match="derivative"):
             ops.paged_attention_decode(dual[:, 0], k_cache, v_cache, table, start)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", [0, 1])
+def test_append_refuses_learned_rotations(device, which):
+    """Tables that require a gradient would get none: the GPU's queries carried
+    no graph where the CPU's did."""
+    k_cache, v_cache = torch.zeros(2, 4, 1, 8, 16, device=device)
+    table = torch.zeros(3, 1, dtype=torch.int32, device=device)
+    start = torch.zeros(3, dtype=torch.int32, device=device)
+    k = torch.zeros(3, 1, 1, 16, device=device)
+    rope = list(ops.rotary_table(8, 16, device=device))
+    rope[which].requires_grad_()
+    with pytest.raises(ValueError, match="rope requires a gradient"):
+        ops.paged_kv_append(k, k, k_cache, v_cache, table, start, q=k, rope=tuple(rope))
+    with torch.no_grad():
+        assert ops.paged_kv_append(k, k, k_cache, v_cache, table, start, q=k, rope=tuple(rope)).shape == k.shape
