@@ -195,8 +195,8 @@ def token_policy_loss(
     count = w.sum().clamp(min=1) if reduction == "mean" else 1.0
     objective = -(gain * w).sum() / count
     # a term without weight is left out: 0 with a gradient of 0, whatever it holds
-    nothing = lp.masked_fill(torch.ones_like(gone), 0.0).sum()
-    kl, loss_kl, entropy = nothing.detach(), nothing, nothing
+    loss_kl, entropy = (lp.masked_fill(torch.ones_like(gone), 0.0).sum() for _ in range(2))
+    kl = torch.zeros_like(objective)
     if ref_log_probs is not None:
         y = torch.where(gone, 0.0, ref_log_probs.float() - lp)
         kl = ((torch.expm1(y) - y) * w).sum() / count

@@ -447,6 +447,19 @@ def test_policy_loss_outputs_change_in_place(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grad", [False, True])
+def test_policy_loss_outputs_are_each_their_own(device, grad):
+    """Absent terms too: a change of one in place leaves the others."""
+    lp = torch.zeros(2, 3, device=device, requires_grad=grad)
+    out = ops.token_policy_loss(lp, torch.zeros(2, 3, device=device), torch.ones(2, 1, device=device))
+    for i in range(7):
+        before = [float(x.detach()) for x in out]
+        out[i].detach().add_(1.0)
+        after = [float(x.detach()) for x in out]
+        assert after == [x + (j == i) for j, x in enumerate(before)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_policy_loss_refusals(device):
     lp = torch.zeros(2, 3, device=device)
     adv = torch.zeros(2, 1, device=device)
