@@ -88,9 +88,10 @@ def token_log_probs(
     Returns:
         ``[...]`` float32.  Differentiable in ``logits``; the gradient has
         the logits' dtype, and is itself differentiable in elementary operations
-        (``create_graph``); forward derivatives (dual tensors) take these as well.  A place with an upstream gradient of 0 gets a
-        gradient of exactly 0 whatever its logits hold.  A row of nothing but
-        ``-inf`` gives NaN.
+        (``create_graph``), which dual tensors take as well for their forward
+        derivatives.  A place with an upstream gradient of 0 gets a gradient of
+        exactly 0 whatever its logits hold.  A row of nothing but ``-inf`` gives
+        NaN.
     """
     c = _native(logits)
     if c is not None:
@@ -161,9 +162,10 @@ def token_policy_loss(
             or float16, any strides.  Only ``log_probs`` gets a gradient; the
             others must not require one.
         advantage: broadcasts to ``log_probs``.
-        mask: bool, integer or float weights of ``log_probs``' shape, taken in float32.  A place
-            of weight 0 may hold anything (the losses' gradient there is 0),
-            though what it holds still enters ``clip_fraction`` and ``ess``.
+        mask: bool, integer or float weights of ``log_probs``' shape, taken in
+            float32.  A place of weight 0 may hold anything (the losses' gradient
+            there is 0), though what it holds still enters ``clip_fraction`` and
+            ``ess``.
         reduction: ``"mean"`` as above, or ``"sum"``: the weighted sums, not
             divided.
     """
