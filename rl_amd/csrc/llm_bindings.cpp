@@ -317,8 +317,17 @@ Tensor log_probs_raw(const Tensor& logits, const Tensor& tokens, double temperat
   return lp;
 }
 
+// Whether a backward pass is left to elementary operations: where it is
+// differentiated in turn (create_graph), and where upstream gradients are many at
+// once (is_grads_batched), wrappers without memory of their own.
+bool plain_backward(const torch::autograd::variable_list& grads) {
+  return at::GradMode::is_enabled() ||
+         std::any_of(grads.begin(), grads.end(),
+                     [](const Tensor& g) { return g.defined() && !g.has_storage(); });
+}
+
 // The gradient (one-hot - softmax) * upstream / temperature in elementary
-// operations, for a caller who differentiates it in turn.
+// operations.
 Tensor log_probs_grad_plain(const Tensor& logits, const Tensor& tokens, const Tensor& upstream,
                             double temperature, int64_t ignore_index) {
   const Tensor gone = tokens.eq(ignore_index);
@@ -327,11 +336,12 @@ Tensor log_probs_grad_plain(const Tensor& logits, const Tensor& tokens, const Te
   Tensor x = logits.to(torch::kFloat32) / temperature;
   // rows that pass nothing back may hold anything, and no NaN comes through them
   const Tensor finite = x.detach().logsumexp(-1).isfinite();
-  const Tensor out = gone.logical_or(g.detach().eq(0).logical_and(finite.logical_not()));
+  const Tensor out = gone.logical_or(g.eq(0).logical_and(finite.logical_not()));
   x = x.masked_fill(out.unsqueeze(-1), 0);
   const Tensor at = tokens.to(torch::kInt64).masked_fill(known.logical_not(), 0).unsqueeze(-1);
-  const Tensor hot = torch::zeros_like(x.detach()).scatter_(-1, at, 1);
-  const Tensor row = known.logical_or(gone).logical_or(g.detach().eq(0));
+  const Tensor hot =
+      torch::zeros(logits.sizes(), logits.options().dtype(torch::kFloat32)).scatter_(-1, at, 1);
+  const Tensor row = known.logical_or(gone).logical_or(g.eq(0));
   const Tensor d = (hot - x.softmax(-1)) * (g.masked_fill(row.logical_not(), NAN) / temperature).unsqueeze(-1);
   return d.to(logits.scalar_type());
 }
@@ -355,7 +365,7 @@ class TokenLogProbs : public torch::autograd::Function<TokenLogProbs> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &stats = saved[2];
     c10::DeviceGuard guard(logits.device());
-    if (at::GradMode::is_enabled())  // create_graph
+    if (plain_backward(grads))
       return {log_probs_grad_plain(logits, saved[1], grads[0],
                                    ctx->saved_data["temperature"].toDouble(),
                                    ctx->saved_data["ignore_index"].toInt()),
@@ -460,8 +470,7 @@ std::vector<Tensor> scalars_of(const Tensor& out, int first, int last) {
   return s;
 }
 
-// The gradient in elementary operations, in double, for a caller who
-// differentiates it in turn: by the log-probs and by the upstream gradients `g`
+// The gradient in elementary operations, in double, for the upstream gradients `g`
 // (undefined: none) of the five scalars.  `factor` is the 1 / D of the means.
 Tensor policy_grad_plain(const Tensor& log_probs, const Tensor& old_log_probs,
                          const Tensor& advantage, const Tensor& mask, const Tensor& ref,
@@ -520,7 +529,7 @@ class TokenPolicyLoss : public torch::autograd::Function<TokenPolicyLoss> {
     const auto saved = ctx->get_saved_variables();
     const auto cfg = ctx->saved_data["config"].toDoubleVector();
     const PolicyConfig c{(int64_t)cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5] != 0.0};
-    if (at::GradMode::is_enabled()) {  // create_graph
+    if (plain_backward(grads)) {
       c10::DeviceGuard guard(saved[0].device());
       none[0] = policy_grad_plain(saved[0], saved[1], saved[2], saved[3], saved[4],
                                   saved[5].select(0, 7), c,

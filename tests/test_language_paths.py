@@ -622,6 +622,36 @@ def test_tracers_and_dispatch_modes_keep_the_plain_form():
         assert any("exp" in n or "log_softmax" in n for n in mode.names)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_batched_gradients(create_graph):
+    """Many upstream gradients in one backward pass, as vectorized Jacobians take
+    them: each equals its own pass."""
+    from rl_amd.modules.llm.transformers_wrapper import _log_probs_of
+
+    g = torch.Generator().manual_seed(11)
+    logits = torch.randn(3, 5, 17, generator=g).cuda().requires_grad_()
+    tokens = torch.randint(0, 17, (3, 5), generator=g).cuda()
+    lp = _log_probs_of(logits, tokens)
+    ups = torch.randn(4, 3, 5, generator=g).cuda()
+    ups[1, 2] = 0
+    (got,) = torch.autograd.grad(lp, logits, ups, is_grads_batched=True, create_graph=create_graph, retain_graph=True)
+    for i in range(4):
+        (want,) = torch.autograd.grad(lp, logits, ups[i], retain_graph=True)
+        assert torch.allclose(got[i], want, atol=1e-6)
+
+    d = grpo_data()
+    x = d["new"].clone().requires_grad_()
+    vals = GRPOLoss(Given(x), kl_to_ref_coeff=0.1, entropy_coeff=0.02)(grpo_td(d, d["mask"] < 0.7))
+    names = ("loss_objective", "loss_kl_to_ref", "loss_entropy", "ESS")
+    losses = [vals.get(k) for k in names]
+    (got,) = torch.autograd.grad(losses, x, [row for row in torch.eye(4, device="cuda")],
+                                 is_grads_batched=True, create_graph=create_graph, retain_graph=True)
+    for i in range(4):
+        (want,) = torch.autograd.grad(losses[i], x, retain_graph=True)
+        assert torch.allclose(got[i], want, atol=1e-6), names[i]
+
+
 # --------------------------------------------------------------------------- #
 # streams, graphs, far offsets
 # --------------------------------------------------------------------------- #
